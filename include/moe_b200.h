@@ -63,6 +63,9 @@ extern "C" {
  * (moe_fp8_row_bytes). Accepted by moe_ep_pack*, moe_p2p_dispatch and
  * moe_p2p_combine_experts_back. */
 #define MOE_DTYPE_E4M3_ROW 3
+/* Latent cache pages in e4m3 with power-of-two block scales (cache_fmt only; the 16-bit
+ * formats are MOE_DTYPE_BF16 and MOE_DTYPE_FP16). */
+#define MOE_CACHE_E4M3 4
 
 /* Human-readable name of a status code (static string). */
 MOE_API const char* moe_status_string(int status);
@@ -444,6 +447,81 @@ MOE_API int moe_ep_pack_mapped(int dtype, const void* hidden_states, const int32
                                int num_experts, const int32_t* expert_map, int world, int32_t* scratch,
                                const int32_t* offsets, void* send_x, int32_t* send_meta, int32_t* tok_rows,
                                void* stream);
+
+/*
+ * Paged latent cache (no reference counterpart: the attention half of the layer whose MoE half
+ * the entry points above are). A cached token is 512 latent values, keys and values of all
+ * heads, and a rotary key of 64.
+ *   16-bit pages  [page_size][576] elements
+ *   MOE_CACHE_E4M3 pages of page_size * 644 bytes: codes [page_size][512], rotary keys bf16
+ *                 [page_size][64], UE8M0 scale bytes [page_size][4] (one scale per 128 values)
+ * page_size is 16, 32, 64 or 128. moe_latent_cache_page_bytes returns -1 for anything else.
+ */
+MOE_API int64_t moe_latent_cache_page_bytes(int cache_fmt, int page_size);
+
+/* Writes num_tokens rows (latent [n, 512] and k_rope [n, 64] of `dtype`, row pitches in
+ * elements, any alignment of the type) to slots[i] = page * page_size + offset; negative slots
+ * are skipped, slots past the cache are skipped and recorded in `status`. 16-bit pages take
+ * their own dtype, e4m3 pages bf16. Two rows for one slot: one of them is kept. */
+MOE_API int moe_latent_cache_write(int dtype, const void* latent, int64_t ld_latent, const void* k_rope,
+                                   int64_t ld_rope, const int64_t* slots, int64_t num_tokens, int cache_fmt,
+                                   void* cache, int64_t num_pages, int page_size, int* status, void* stream);
+
+/* Reads contexts back as contiguous rows: row cu_lens[b] + j of latent [total, 512] and k_rope
+ * [total, 64] is position j of request b, in the cache's type (bf16 from e4m3 pages). Rows past
+ * cu_lens[num_seqs] are zeros; positions whose page is outside the cache or past the table read
+ * as NaN and are recorded in `status`. block_table int32 [num_seqs, table_width], pitch ld_table. */
+MOE_API int moe_latent_cache_read(int cache_fmt, const void* cache, int64_t num_pages, int page_size,
+                                  const int32_t* block_table, int64_t ld_table, int table_width,
+                                  const int32_t* cu_lens, int num_seqs, int64_t total, void* latent, void* k_rope,
+                                  int* status, void* stream);
+
+/*
+ * Latent attention over the paged cache, absorbed form: query row (b, i, h) of q [num_seqs, q_len,
+ * heads, 576] attends to positions j <= cache_lens[b] - q_len + i of its request,
+ *   out = sum_j softmax_j(scale q . [c_j, r_j]) c_j   [num_seqs, q_len, heads, 512]
+ * and lse (optional, fp32 [num_seqs, q_len, heads]) is the natural log of the softmax sum. Rows
+ * that see nothing give zeros and -inf. cache_lens past the table are cut to it and recorded in
+ * `status`, pages outside the cache are left out and recorded. q_len * heads <= 65536.
+ */
+MOE_API size_t moe_latent_decode_workspace_bytes(int64_t num_seqs, int q_len, int heads);
+MOE_API int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int q_len, int heads, int cache_fmt,
+                              const void* cache, int64_t num_pages, int page_size, const int32_t* block_table,
+                              int64_t ld_table, int table_width, const int32_t* cache_lens, float scale, void* out,
+                              float* lse, void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * Latent attention, expanded form, over requests of different lengths: q [total_q, heads, 192],
+ * kv [total_k, heads, 256] (keys' 128 without position, then values' 128: the up-projection's
+ * output), k_rope [total_k, 64] shared by the heads; strides in elements (multiples of 8), last
+ * dimension contiguous. Request b has query rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] ..
+ * cu_k[b + 1]; with `causal` its last query sees all its keys, the one before one key less, and
+ * so on. out [total_q, heads, 128], lse (optional) fp32 [total_q, heads]; rows that see nothing,
+ * and rows past cu_q[num_seqs], give zeros and -inf.
+ */
+MOE_API int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
+                               int64_t kv_stride_t, int64_t kv_stride_h, const void* k_rope, int64_t kr_stride_t,
+                               const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int64_t total_q,
+                               int64_t total_k, int heads, float scale, int causal, void* out, float* lse,
+                               int* status, void* stream);
+
+/*
+ * A whole MoE layer for a few tokens in two kernels: the routing of moe_grouped_topk on
+ * gating_output, then sum over the chosen experts of weight * W2 (silu(W1g x) * W1u x), every
+ * chosen expert's weights read once. Weights in the tokens' type, or with weight_e4m3 in e4m3
+ * with fp32 scales per 128 x 128 block (moe_quantize_blocks_fp8); the tokens keep 16 bits.
+ * num_tokens <= moe_few_max_tokens(topk) (32, less when topk > 16). ld_hidden: row pitch of
+ * hidden_states in elements, a multiple of 8. A token whose logits give no order (NaN) gets NaN.
+ */
+MOE_API int moe_few_max_tokens(int topk);
+MOE_API size_t moe_few_workspace_bytes(int64_t num_tokens, int topk, int intermediate_size);
+MOE_API int moe_few_tokens(int dtype, const void* hidden_states, int64_t ld_hidden, const float* gating_output,
+                           const float* bias, int weight_e4m3, const void* w1, const float* w1_scale,
+                           const void* w2, const float* w2_scale, int64_t num_tokens, int num_experts, int topk,
+                           int renormalize, int num_expert_group, int topk_group, int scoring_func,
+                           int group_score_mode, float routed_scaling_factor, int hidden_size,
+                           int intermediate_size, void* out, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,7 @@ Public API (mirrors the reference's task signatures):
 
 Drop-in task modules with the reference harness contract (``ModelNew``,
 ``get_inputs``, ``get_init_inputs``) live in ``tasks/``; the expert-parallel
-layer is in ``ep``. Importing the package also registers the operators as
+layer is in ``ep``, latent attention over a paged latent cache in ``attention``. Importing the package also registers the operators as
 ``torch.ops.moe_b200.*`` (``torch_ops``).
 """
 
@@ -24,6 +24,8 @@ from .ops import (  # noqa: F401
     grouped_topk,
     is_ue8m0,
     moe_align,
+    moe_decode,
+    moe_decode_max_tokens,
     moe_layer,
     quantize_rows_fp8,
     quantize_rows_fp8_packed,
@@ -33,9 +35,20 @@ from .ops import (  # noqa: F401
     weights_scale_format,
 )
 
+from .attention import (  # noqa: F401
+    latent_attention_decode,
+    latent_attention_decode_workspace_bytes,
+    latent_attention_prefill,
+    latent_cache,
+    latent_cache_read,
+    latent_cache_write,
+)
+
 from . import torch_ops  # noqa: E402,F401  (registers torch.ops.moe_b200.*)
 
 __all__ = ["grouped_topk", "fused_moe", "fused_moe_fp8", "softmax_topk", "moe_align", "moe_layer",
            "fused_moe_workspace_bytes", "quantize_rows_fp8", "quantize_weights_fp8", "check_device_status",
            "router_grouped_topk", "fp8_row_bytes", "quantize_rows_fp8_packed", "fused_moe_fp8_rows",
-           "is_ue8m0", "weights_scale_format"]
+           "is_ue8m0", "weights_scale_format", "moe_decode", "moe_decode_max_tokens", "latent_cache",
+           "latent_cache_write", "latent_cache_read", "latent_attention_decode",
+           "latent_attention_decode_workspace_bytes", "latent_attention_prefill"]

@@ -33,6 +33,7 @@ MOE_DTYPE_BF16 = 0
 MOE_DTYPE_FP16 = 1
 MOE_DTYPE_FP32 = 2
 MOE_DTYPE_E4M3_ROW = 3
+MOE_CACHE_E4M3 = 4
 MOE_FP8_SCALE_FP32 = 0
 MOE_FP8_SCALE_UE8M0 = 1
 
@@ -99,6 +100,19 @@ SIGNATURES = {
     "moe_ep_plan_mapped": (_i32, [_c_p, _i64, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p]),
     "moe_ep_pack_mapped": (_i32, [_i32, _c_p, _c_p, _c_p, _i64, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p, _c_p, _c_p,
                                   _c_p, _c_p]),
+    "moe_latent_cache_page_bytes": (_i64, [_i32, _i32]),
+    "moe_latent_cache_write": (_i32, [_i32, _c_p, _i64, _c_p, _i64, _c_p, _i64, _i32, _c_p, _i64, _i32, _c_p, _c_p]),
+    "moe_latent_cache_read": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _i64, _i32, _c_p, _i32, _i64, _c_p, _c_p, _c_p,
+                                     _c_p]),
+    "moe_latent_decode_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "moe_latent_decode": (_i32, [_i32, _c_p, _i64, _i32, _i32, _i32, _c_p, _i64, _i32, _c_p, _i64, _i32, _c_p, _f32,
+                                 _c_p, _c_p, _c_p, _sz, _c_p, _c_p]),
+    "moe_latent_prefill": (_i32, [_i32, _c_p, _i64, _i64, _c_p, _i64, _i64, _c_p, _i64, _c_p, _c_p, _i32, _i64, _i64,
+                                  _i32, _f32, _i32, _c_p, _c_p, _c_p, _c_p]),
+    "moe_few_max_tokens": (_i32, [_i32]),
+    "moe_few_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "moe_few_tokens": (_i32, [_i32, _c_p, _i64, _c_p, _c_p, _i32, _c_p, _c_p, _c_p, _c_p, _i64, _i32, _i32, _i32, _i32,
+                              _i32, _i32, _i32, _f32, _i32, _i32, _c_p, _c_p, _sz, _c_p]),
     "moe_ep_combine": (_i32, [_i32, _c_p, _c_p, _i64, _i32, _i32, _c_p, _c_p]),
 }
 

@@ -350,4 +350,143 @@ __device__ __forceinline__ void route_token_lanes(const float* row, const float*
                                scale, out_w, out_ids, scr);
 }
 
+constexpr int kRouteMaxExperts = 512;
+
+struct RouteCand {
+  float v;    // ranking value (choice)
+  int idx;    // expert index (INT_MAX when empty)
+  float s;    // unbiased score (the weight before renormalisation)
+};
+
+__device__ __forceinline__ RouteCand route_warp_best(RouteCand c) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    RouteCand o;
+    o.v = __shfl_xor_sync(0xffffffffu, c.v, off);
+    o.idx = __shfl_xor_sync(0xffffffffu, c.idx, off);
+    o.s = __shfl_xor_sync(0xffffffffu, c.s, off);
+    if (route_better(o.v, o.idx, c.v, c.idx)) c = o;
+  }
+  return c;
+}
+
+// One token's routing by one warp for any E <= 32 * VPL and any group size: group scores go
+// through the warp's shared row s_choice (E floats).
+template <int VPL, bool VEC>
+__device__ __forceinline__ void route_token_general(const float* __restrict__ row, const float* __restrict__ bias,
+                                                    int64_t tok, int E, int topk, int renormalize, int n_group,
+                                                    int topk_group, int scoring, int gmode, float scale,
+                                                    float* __restrict__ out_w, int32_t* __restrict__ out_ids,
+                                                    float* s_choice) {
+  const int lane = threadIdx.x & 31;
+  const int e0 = lane * VPL;
+  float x[VPL];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < VPL; i += 4) {
+      if (e0 + i < E) {
+        float4 v = __ldg(reinterpret_cast<const float4*>(row + e0 + i));
+        x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+      } else {
+        x[i] = x[i + 1] = x[i + 2] = x[i + 3] = -INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) x[i] = (e0 + i < E) ? __ldg(row + e0 + i) : -INFINITY;
+  }
+
+  // scores (v0 :98-103)
+  float s[VPL];
+  if (scoring == MOE_SCORING_SOFTMAX) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) m = fmaxf(m, x[i]);
+    m = route_warp_max(m);
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      s[i] = (e0 + i < E) ? expf(x[i] - m) : 0.f;
+      z += s[i];
+    }
+    z = route_warp_sum(z);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s[i] = s[i] / z;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) s[i] = 1.0f / (1.0f + expf(-x[i]));
+  }
+
+  // ranking values
+  float c[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const bool valid = e0 + i < E;
+    c[i] = valid ? (bias ? s[i] + __ldg(bias + e0 + i) : s[i]) : -INFINITY;
+  }
+
+  // group selection (v0 :109-123)
+  const int epg = E / n_group;
+  if (topk_group < n_group) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e0 + i < E) s_choice[e0 + i] = c[i];
+    __syncwarp();
+    float gs = -INFINITY;
+    if (lane < n_group) {
+      const float* gp = &s_choice[lane * epg];
+      if (gmode == MOE_GROUP_SCORE_MAX) {
+        for (int j = 0; j < epg; ++j) gs = fmaxf(gs, gp[j]);
+      } else {
+        float b1 = -INFINITY, b2 = -INFINITY;
+        for (int j = 0; j < epg; ++j) {
+          const float v = gp[j];
+          if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) { b2 = v; }
+        }
+        gs = b1 + b2;
+      }
+    }
+    int rank = 0;
+    for (int h = 0; h < n_group; ++h) {
+      const float o = __shfl_sync(0xffffffffu, gs, h);
+      rank += (o > gs) || (o == gs && h < lane);
+    }
+    const unsigned keep = __ballot_sync(0xffffffffu, lane < n_group && rank < topk_group);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = e0 + i;
+      if (e < E && !((keep >> (e / epg)) & 1u)) c[i] = -INFINITY;
+    }
+  }
+
+  // top-k rounds (v0 :124)
+  unsigned taken = 0;
+  float my_w = 0.f;
+  int my_id = 0;
+  for (int r = 0; r < topk; ++r) {
+    RouteCand b{-INFINITY, INT_MAX, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = e0 + i;
+      if (e < E && !((taken >> i) & 1u) && route_better(c[i], e, b.v, b.idx)) {
+        b.v = c[i]; b.idx = e; b.s = s[i];
+      }
+    }
+    b = route_warp_best(b);
+    if (b.idx >= e0 && b.idx < e0 + VPL) taken |= 1u << (b.idx - e0);
+    if (lane == r) { my_w = b.s; my_id = b.idx; }
+  }
+
+  // renormalise and scale (v0 :126-130)
+  if (renormalize) {
+    const float tot = route_warp_sum(lane < topk ? my_w : 0.f);
+    my_w = my_w / tot;
+  }
+  if (scale != 1.0f) my_w *= scale;
+  if (lane < topk) {
+    out_w[tok * topk + lane] = my_w;
+    out_ids[tok * topk + lane] = my_id;
+  }
+}
+
 }  // namespace moe

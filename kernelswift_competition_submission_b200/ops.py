@@ -524,3 +524,85 @@ def moe_layer(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, n
     w, ids = grouped_topk(hidden_states, gating_output, topk, renormalize, num_expert_group, topk_group,
                           scoring_func, routed_scaling_factor, e_score_correction_bias)
     return fused_moe(hidden_states, w1, w2, w, ids)
+
+
+def moe_decode_max_tokens(topk: int) -> int:
+    """The largest batch ``moe_decode`` takes: 32 tokens, fewer when topk is above 16."""
+    return int(_lib.load().moe_few_max_tokens(int(topk)))
+
+
+def moe_decode(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, num_expert_group=1, topk_group=1,
+               scoring_func="softmax", routed_scaling_factor=1.0, e_score_correction_bias=None, group_score=None,
+               w1_scale=None, w2_scale=None, out=None, workspace=None):
+    """``moe_layer`` for the few tokens of a decode step, in two kernels that read every chosen
+    expert's weights once.
+
+    hidden_states [M, K] (bf16 or fp16, M <= ``moe_decode_max_tokens(topk)``), gating_output
+    [M, E]; w1 [E, 2N, K] and w2 [E, K, N] in the dtype of hidden_states, or e4m3 with fp32
+    ``w1_scale`` / ``w2_scale`` per 128 x 128 block (``quantize_weights_fp8``). With e4m3 weights
+    the tokens and SiLU*mul rows keep their 16 bits (``fused_moe_fp8`` quantises them). Routing
+    as ``grouped_topk``. Returns [M, K] in the dtype of hidden_states.
+    """
+    name = "moe_decode"
+    if scoring_func == "softmax":
+        sf = _lib.MOE_SCORING_SOFTMAX
+    elif scoring_func == "sigmoid":
+        sf = _lib.MOE_SCORING_SIGMOID
+    else:
+        raise ValueError(f"Unsupported scoring_func: {scoring_func}")
+    if group_score is None:
+        group_score = "max" if e_score_correction_bias is None else "top2sum"
+    gm = {"max": _lib.MOE_GROUP_SCORE_MAX, "top2sum": _lib.MOE_GROUP_SCORE_TOP2_SUM}[group_score]
+    dev = _require_cuda(name, hidden_states, gating_output, w1, w2, e_score_correction_bias, w1_scale, w2_scale)
+    dt = hidden_states.dtype
+    if dt not in _DTYPES:
+        raise TypeError(f"{name}: hidden_states dtype {dt} not supported (bf16 or fp16)")
+    if hidden_states.dim() != 2 or gating_output.dim() != 2 or w1.dim() != 3 or w2.dim() != 3:
+        raise ValueError(f"{name}: hidden_states [M, K], gating_output [M, E], w1 [E, 2N, K], w2 [E, K, N]")
+    M, K = hidden_states.shape
+    E, twoN, K1 = w1.shape
+    N = twoN // 2
+    if K1 != K or twoN != 2 * N or tuple(w2.shape) != (E, K, N):
+        raise ValueError(f"{name}: shape mismatch x{tuple(hidden_states.shape)} w1{tuple(w1.shape)} "
+                         f"w2{tuple(w2.shape)}")
+    if tuple(gating_output.shape) != (M, E):
+        raise ValueError(f"{name}: gating_output must be [{M}, {E}]")
+    f8 = w1.dtype in (torch.float8_e4m3fn, torch.uint8)
+    s1 = s2 = None
+    if f8:
+        w1, w2 = _fp8_bytes(w1), _fp8_bytes(w2)
+        if w1_scale is None or w2_scale is None:
+            raise ValueError(f"{name}: e4m3 weights need w1_scale and w2_scale")
+        if tuple(w1_scale.shape) != (E, twoN // 128, K // 128) or tuple(w2_scale.shape) != (E, K // 128, N // 128):
+            raise ValueError(f"{name}: scales must be [E, rows / 128, columns / 128]")
+        s1, s2 = w1_scale.to(torch.float32).contiguous(), w2_scale.to(torch.float32).contiguous()
+    elif w1.dtype != dt or w2.dtype != dt:
+        raise TypeError(f"{name}: w1/w2 must have the dtype of hidden_states, or be e4m3")
+    lib = _lib.load()
+    if M > int(lib.moe_few_max_tokens(topk)):
+        raise ValueError(f"{name}: at most {int(lib.moe_few_max_tokens(topk))} tokens at topk {topk}, got {M}; "
+                         "use moe_layer or grouped_topk with fused_moe_fp8")
+    x = hidden_states
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+    g = gating_output.to(torch.float32).contiguous()
+    bias = None
+    if e_score_correction_bias is not None:
+        bias = e_score_correction_bias.to(torch.float32).contiguous()
+        if bias.numel() != E:
+            raise ValueError(f"{name}: e_score_correction_bias must have {E} values")
+    w1, w2 = w1.contiguous(), w2.contiguous()
+    if out is None:
+        out = torch.empty(M, K, dtype=dt, device=dev)
+    elif tuple(out.shape) != (M, K) or out.dtype != dt or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"{name}: out must be a contiguous {dt} [{M}, {K}] tensor on {dev}")
+    need = int(lib.moe_few_workspace_bytes(M, topk, N))
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+    _lib.check(
+        lib.moe_few_tokens(_DTYPES[dt], _ptr(x), x.stride(0), _ptr(g), _ptr(bias), int(f8), _ptr(w1), _ptr(s1),
+                           _ptr(w2), _ptr(s2), M, E, topk, int(bool(renormalize)), num_expert_group, topk_group, sf,
+                           gm, float(routed_scaling_factor), K, N, _ptr(out), _ptr(workspace),
+                           workspace.numel() * workspace.element_size(), _stream(dev)),
+        "moe_few_tokens")
+    return out
