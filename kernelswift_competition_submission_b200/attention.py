@@ -170,9 +170,13 @@ def latent_attention_decode_workspace_bytes(num_requests: int, n_q: int, heads: 
     return int(_lib.load().moe_latent_decode_workspace_bytes(num_requests, n_q, heads))
 
 
-def _strided3(t: torch.Tensor) -> torch.Tensor:
-    ok = t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
+def _tma_rows(t: torch.Tensor) -> torch.Tensor:
+    """t itself when TMA can read it (16-byte aligned rows, no broadcast), else a contiguous copy.
+    The strides of dimensions of one are never used."""
+    ok = t.data_ptr() % 16 == 0 and t.stride(-1) == 1
+    for n, st in zip(t.shape[:-1], t.stride()[:-1]):
+        ok = ok and (n <= 1 or (st > 0 and st % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def latent_attention_prefill(q, kv, k_rope, cu_q, cu_k, scale, *, causal=True, out=None, return_lse=False):
@@ -203,9 +207,7 @@ def latent_attention_prefill(q, kv, k_rope, cu_q, cu_k, scale, *, causal=True, o
     cu_q, cu_k = _ints(name, "cu_q", cu_q), _ints(name, "cu_k", cu_k)
     if cu_q.shape[0] < 1 or cu_q.shape != cu_k.shape:
         raise ValueError(f"{name}: cu_q and cu_k must have the same length, requests + 1")
-    q, kv = _strided3(q), _strided3(kv)
-    if k_rope.stride(1) != 1 or k_rope.stride(0) % 8 or k_rope.data_ptr() % 16:
-        k_rope = k_rope.contiguous()
+    q, kv, k_rope = _tma_rows(q), _tma_rows(kv), _tma_rows(k_rope)
     if out is None:
         out = torch.empty(tq, heads, NOPE_DIM, dtype=dt, device=dev)
     elif tuple(out.shape) != (tq, heads, NOPE_DIM) or out.dtype != dt or not out.is_contiguous() or out.device != dev:

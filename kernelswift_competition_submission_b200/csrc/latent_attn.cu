@@ -108,58 +108,6 @@ latent_decode_rows_kernel(const T* __restrict__ q, const uint8_t* __restrict__ c
   if (lse != nullptr && lane == 0) lse[row] = l > 0.f || l != l ? m + logf(l) : -INFINITY;
 }
 
-__device__ __forceinline__ int find_seq(const int32_t* __restrict__ cu, int n, int64_t i) {
-  int lo = 0, hi = n;  // the last b with cu[b] <= i
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int64_t)__ldg(cu + mid) <= i) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kRowsPerBlock)
-latent_prefill_rows_kernel(const T* __restrict__ q, int64_t q_st, int64_t q_sh, const T* __restrict__ kv, int64_t kv_st,
-                           int64_t kv_sh, const T* __restrict__ k_rope, int64_t kr_st, const int32_t* __restrict__ cu_q,
-                           const int32_t* __restrict__ cu_k, int num_seqs, int64_t tq, int64_t tk, int heads,
-                           float scale, bool causal, T* __restrict__ out, float* __restrict__ lse) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + (threadIdx.x >> 5);
-  if (row >= tq * heads) return;
-  const int64_t t = row / heads;
-  const int h = (int)(row - t * heads);
-  const int b = find_seq(cu_q, num_seqs, t);
-  float qv[6];
-#pragma unroll
-  for (int i = 0; i < 6; ++i) qv[i] = ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(q + t * q_st + h * q_sh + 32 * i + lane)).x;
-  int64_t seen = 0, k0 = 0;
-  if (b < num_seqs) {
-    k0 = __ldg(cu_k + b);
-    const int64_t nk = min((int64_t)__ldg(cu_k + b + 1), tk) - k0, nq = __ldg(cu_q + b + 1) - __ldg(cu_q + b);
-    seen = causal ? min(nk, nk - nq + 1 + (t - __ldg(cu_q + b))) : nk;
-  }
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t j = 0; j < seen; ++j) {
-    const T* kp = kv + (k0 + j) * kv_st + h * kv_sh;
-    float s = 0.f, v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s = fmaf(qv[i], ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(kp + 32 * i + lane)).x, s);
-      v[i] = ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(kp + kNopeDim + 32 * i + lane)).x;
-    }
-#pragma unroll
-    for (int i = 4; i < 6; ++i)
-      s = fmaf(qv[i], ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(k_rope + (k0 + j) * kr_st + 32 * (i - 4) + lane)).x, s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    online_step(s * scale, v, m, l, acc);
-  }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[row * kNopeDim + 32 * i + lane] = ElemTraits<T>::from_float(acc[i] * inv);
-  if (lse != nullptr && lane == 0) lse[row] = l > 0.f || l != l ? m + logf(l) : -INFINITY;
-}
-
 inline bool al(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
@@ -201,37 +149,5 @@ extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int
   else if (dtype == MOE_DTYPE_BF16) MOE_LD(__nv_bfloat16, false);
   else MOE_LD(__half, false);
 #undef MOE_LD
-  return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
-}
-
-extern "C" int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
-                                  int64_t kv_stride_t, int64_t kv_stride_h, const void* k_rope, int64_t kr_stride_t,
-                                  const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int64_t total_q,
-                                  int64_t total_k, int heads, float scale, int causal, void* out, float* lse,
-                                  int* status, void* stream) {
-  using namespace moe;
-  if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_FP16) return MOE_ERR_UNSUPPORTED;
-  if (num_seqs < 0 || total_q < 0 || total_k < 0 || heads <= 0) return MOE_ERR_INVALID_ARG;
-  if (q_stride_t < 0 || q_stride_h < 0 || kv_stride_t < 0 || kv_stride_h < 0 || kr_stride_t < 0)
-    return MOE_ERR_INVALID_ARG;
-  if (total_q > INT32_MAX || total_k > INT32_MAX || heads > 65535 || num_seqs > 65535) return MOE_ERR_BAD_SHAPE;
-  if (total_q == 0) return MOE_OK;
-  if (!q || !cu_q || !cu_k || !out || (total_k > 0 && (!kv || !k_rope))) return MOE_ERR_INVALID_ARG;
-  if (!al(q, 16) || !al(kv, 16) || !al(k_rope, 16) || !al(out, 16)) return MOE_ERR_INVALID_ARG;
-  if (q_stride_t % 8 || q_stride_h % 8 || kv_stride_t % 8 || kv_stride_h % 8 || kr_stride_t % 8)
-    return MOE_ERR_BAD_SHAPE;
-  const int rc = moe_check_device();
-  if (rc != MOE_OK) return rc;
-  (void)status;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t nb = ceil_div(total_q * heads, kRowsPerBlock);
-  if (nb > INT32_MAX) return MOE_ERR_BAD_SHAPE;
-#define MOE_LP(T)                                                                                              \
-  latent_prefill_rows_kernel<T><<<(unsigned)nb, 32 * kRowsPerBlock, 0, st>>>(                                  \
-      static_cast<const T*>(q), q_stride_t, q_stride_h, static_cast<const T*>(kv), kv_stride_t, kv_stride_h,   \
-      static_cast<const T*>(k_rope), kr_stride_t, cu_q, cu_k, num_seqs, total_q, total_k, heads, scale, causal != 0,    \
-      static_cast<T*>(out), lse)
-  if (dtype == MOE_DTYPE_BF16) MOE_LP(__nv_bfloat16); else MOE_LP(__half);
-#undef MOE_LP
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }

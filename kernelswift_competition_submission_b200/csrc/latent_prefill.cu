@@ -1,0 +1,562 @@
+// Latent attention, expanded form, on the tensor cores (tcgen05 + TMEM + TMA).
+//
+//   s_ij = scale (q_i[0:128] . k_j + q_i[128:192] . r_j),  o_i = sum_j softmax_j(s_ij) v_j
+// over the keys j that query i of its request sees; k, v per head, the rotary key r shared.
+//
+// One CTA takes 256 query rows of one head as two 128-row subtiles and walks the keys 128 at a
+// time with a running maximum and sum per row:
+//   warps 0-3, 4-7  softmax of subtile 0 / 1, one row per thread: S from TMEM into registers,
+//                   maximum, exp2, row sum in fp32, P as 16-bit pairs back into S's columns
+//   warp 8          TMA producer: K as three [128 keys][64] boxes, V as two [64 keys][128] halves,
+//                   16 KB slots in a ring of 8, in the order the MMAs use them
+//   warp 9          MMA issuer: S = Q K^T from shared memory, O += P V with P from TMEM and V as it
+//                   lies (MN-major)
+//   warps 10-11     look at V before its MMAs where a row of the tile may not see a key (see below)
+// The MMAs of one subtile run while the other one's softmax does: after PV of subtile i the next
+// QK of i is issued at once, so its scores wait for the softmax and not the other way round.
+//
+// The reference point of a row's exponentials follows its maximum only when that has moved by
+// more than 2^8: P then stays below 256 (exact range for both 16-bit types), the sum is fp32, and
+// O in TMEM is rescaled a few times per row instead of once per tile. P is rounded to the
+// inputs' type for the second product (as wide as V itself); l sums the unrounded values.
+//
+// Masked places: a score is replaced before the maximum is taken, so keys may hold anything.
+// V meets P = 0 in the MMA, and 0 * NaN is NaN, so warps 10-11 zero the V rows past the request's
+// end, and look for non-finite values in tiles that some row sees only in part; if there is one,
+// the CTA's rows are computed again by the softmax warps, key by key over visible keys only.
+//
+// What bounds it: per 128 keys and CTA the MMAs take 2560 clocks, the exponentials 2048 of the
+// 4-per-clock units of each SM quarter, so the two have to overlap all the time.
+#include "latent.h"
+
+namespace moe {
+namespace {
+
+constexpr int kPfThreads = 384;
+constexpr int kPfTile = 128;             // keys per tile, rows per subtile
+constexpr int kPfSlots = 8;
+constexpr int kSlotBytes = 16384;
+constexpr int kQSubBytes = 3 * 16384;    // a subtile of Q: three [128 rows][64] chunks
+constexpr float kRescaleLog2 = 8.0f;
+
+struct PfSmem {
+  static constexpr int kRing = 2 * kQSubBytes;
+  static constexpr int kBars = kRing + kPfSlots * kSlotBytes;
+  // q, full[8], empty[8], s_full[2], p_full[2], o_full[2], v_ok[2], mma_done
+  static constexpr int kNumBars = 1 + 2 * kPfSlots + 9;
+  static constexpr int kMisc = kBars + kNumBars * 8;
+  static constexpr int kBytes = kMisc + 64 + 1024;
+};
+
+struct PfArgs {
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* kv;
+  int64_t kv_st, kv_sh;
+  const void* kr;
+  int64_t kr_st;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int num_seqs;
+  int64_t tq, tk;
+  int heads, units;
+  float scale;       // natural units, for the row-by-row path
+  float scale_log2;  // |scale| * log2(e), above zero
+  int neg;           // scale below zero: scores change sign first
+  int causal;
+  void* out;
+  float* lse;
+  int* status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// One row by a warp, key by key, over the keys it sees: fp32, online softmax. Lane l holds
+// elements l, l + 32, ... of the 192 and of the 128.
+template <typename T>
+__device__ __noinline__ void prefill_row(const PfArgs& a, int64_t t, int h, int64_t k0, int64_t seen) {
+  const int lane = threadIdx.x & 31;
+  const T* q = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
+  float qv[6];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) qv[i] = ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(q + 32 * i + lane)).x;
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t j = 0; j < seen; ++j) {
+    const T* kp = static_cast<const T*>(a.kv) + (k0 + j) * a.kv_st + h * a.kv_sh;
+    const T* rp = static_cast<const T*>(a.kr) + (k0 + j) * a.kr_st;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+      const T* p = i < 4 ? kp + 32 * i : rp + 32 * (i - 4);
+      s = fmaf(qv[i], ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(p + lane)).x, s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    s *= a.scale;
+    const float mn = fmaxf(m, s);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = expf(m - base), p = expf(s - base);
+    m = mn;
+    l = l * f + p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      acc[i] = acc[i] * f +
+               p * ElemTraits<T>::unpack2(*reinterpret_cast<const uint16_t*>(kp + kNopeDim + 32 * i + lane)).x;
+  }
+  const bool some = l > 0.f || l != l;
+  const float inv = some ? 1.f / l : 0.f;
+  const int64_t row = t * a.heads + h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    static_cast<T*>(a.out)[row * kNopeDim + 32 * i + lane] = ElemTraits<T>::from_float(acc[i] * inv);
+  if (a.lse != nullptr && lane == 0) a.lse[row] = some ? m + logf(l) : -INFINITY;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPfThreads, 1)
+latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
+                      const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ PfArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + PfSmem::kRing;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PfSmem::kBars);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + kPfSlots;
+  uint64_t* s_full = empty + kPfSlots;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* v_ok = o_full + 2;
+  uint64_t* mma_done = v_ok + 2;
+  int* misc = reinterpret_cast<int*>(smem + PfSmem::kMisc);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc);
+  volatile int* s_abort = misc + 1;
+  volatile int* s_bad = misc + 2;
+  int* s_unit = misc + 4;  // request, tile
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x / a.units;
+  const int unit = a.units - 1 - (blockIdx.x - h * a.units);
+
+  // which request and tile: prefix of ceil(rows / 256); the rows past cu_q[num_seqs] are one more
+  // request without keys
+  if (warp == 0) {
+    int base = 0, found = -1, tile = 0;
+    for (int b0 = 0; b0 <= a.num_seqs && found < 0; b0 += 32) {
+      const int b = b0 + lane;
+      int n = 0;
+      if (b <= a.num_seqs) {
+        const int64_t lo = min((int64_t)max(__ldg(a.cu_q + b), 0), a.tq);
+        const int64_t hi = b < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + b + 1), 0), a.tq) : a.tq;
+        n = hi > lo ? (int)((hi - lo + 255) / 256) : 0;
+      }
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, unit < base + inc);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        found = b0 + src;
+        tile = unit - base - __shfl_sync(0xffffffffu, inc - n, src);
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) { s_unit[0] = found; s_unit[1] = tile; }
+  }
+  if (threadIdx.x == 64) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < kPfSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); }
+    mbar_init(mma_done, 1);
+    *s_abort = 0;
+    *s_bad = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int req = s_unit[0];
+  if (req < 0) return;  // past the last unit: nothing allocated, nothing in flight
+  const int64_t q_lo = min((int64_t)max(__ldg(a.cu_q + req), 0), a.tq);
+  const int64_t q_hi = req < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + req + 1), 0), a.tq) : a.tq;
+  const int nq = (int)(q_hi - q_lo);
+  int64_t k_lo = 0;
+  int nk = 0;
+  if (req < a.num_seqs) {
+    k_lo = min((int64_t)max(__ldg(a.cu_k + req), 0), a.tk);
+    const int64_t k_hi = min((int64_t)max(__ldg(a.cu_k + req + 1), 0), a.tk);
+    nk = k_hi > k_lo ? (int)(k_hi - k_lo) : 0;
+  }
+  const int row0 = s_unit[1] * 256;
+  // keys seen by row i of the request, and the tiles each subtile walks
+  auto seen = [&](int i) { return i >= nq ? 0 : (a.causal ? max(0, nk - nq + 1 + i) : nk); };
+  int n_tiles[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int last = min(row0 + i * kPfTile + kPfTile, nq) - 1;  // the subtile's last row
+    n_tiles[i] = last >= row0 + i * kPfTile ? (seen(last) + kPfTile - 1) / kPfTile : 0;
+  }
+  const int n_max = max(n_tiles[0], n_tiles[1]);
+  // tile j needs its V looked at when some row that walks it does not see all of it; row 0's
+  // limit is the smallest, and the last tile may run past the request
+  const int sure = min(nk, a.causal ? max(0, nk - nq + 1 + row0) : nk) / kPfTile;  // tiles all rows see whole
+
+  if (n_max > 0) {
+    if (warp == 9) { tmem_alloc(s_tmem, 512); tmem_relinquish(); }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (n_max == 0) {
+    if (warp < 8) {
+      const int i = row0 + threadIdx.x;
+      if (i < nq) {
+        const int64_t row = (q_lo + i) * a.heads + h;
+        uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * kNopeDim);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (a.lse != nullptr) a.lse[row] = -INFINITY;
+      }
+    }
+    return;
+  }
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer
+      tma_prefetch_desc(&map_q);
+      tma_prefetch_desc(&map_kv);
+      tma_prefetch_desc(&map_kr);
+      mbar_arrive_expect_tx(q_full, 2 * kQSubBytes);
+      for (int i = 0; i < 2; ++i)
+        for (int c = 0; c < 3; ++c)
+          for (int r = 0; r < 2; ++r)
+            tma_load_3d(&map_q, q_full, smem + i * kQSubBytes + c * 16384 + r * 8192, c * 64,
+                        (int)q_lo + row0 + i * kPfTile + r * 64, h);
+      int slot = 0;
+      uint32_t phase = 0, issued = 0, issued_parity = 0;
+      bool ok = true;
+      for (int j = 0; j < n_max && ok; ++j) {
+        const int kt = (int)k_lo + j * kPfTile;
+        for (int c = 0; c < 5; ++c) {
+          if (!mbar_wait(&empty[slot], phase ^ 1, a.status, s_abort)) { ok = false; break; }
+          uint8_t* dst = ring + slot * kSlotBytes;
+          mbar_arrive_expect_tx(&full[slot], kSlotBytes);
+          if (c < 2) {
+            tma_load_3d(&map_kv, &full[slot], dst, c * 64, kt, h);
+            tma_load_3d(&map_kv, &full[slot], dst + 8192, c * 64, kt + 64, h);
+          } else if (c == 2) {
+            tma_load_2d(&map_kr, &full[slot], dst, 0, kt);
+            tma_load_2d(&map_kr, &full[slot], dst + 8192, 0, kt + 64);
+          } else {
+            tma_load_3d(&map_kv, &full[slot], dst, kNopeDim, kt + (c - 3) * 64, h);
+            tma_load_3d(&map_kv, &full[slot], dst + 8192, kNopeDim + 64, kt + (c - 3) * 64, h);
+          }
+          issued |= 1u << slot;
+          issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
+          if (++slot == kPfSlots) { slot = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {  // wait (bounded) for the copies in flight before the CTA may leave
+        mbar_wait(q_full, 0, nullptr, nullptr);
+        for (int s = 0; s < kPfSlots; ++s)
+          if ((issued >> s) & 1u) mbar_wait(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      // ------------------------------------------------ MMA issuer
+      constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
+      constexpr uint32_t kIdescPV = idesc_f16(128, 128, ElemTraits<T>::kFmt) | kIdescBMnMajor;
+      // ring position of tile j's K (0..2) and V (3, 4)
+      auto slot_of = [&](int j, int c) { return (5 * j + c) % kPfSlots; };
+      auto phase_of = [&](int j, int c) { return (uint32_t)((5 * j + c) / kPfSlots) & 1u; };
+      auto wait_slots = [&](int j, int c0, int c1) {
+        for (int c = c0; c < c1; ++c)
+          if (!mbar_wait(&full[slot_of(j, c)], phase_of(j, c), a.status, s_abort)) return false;
+        return true;
+      };
+      auto issue_qk = [&](int i, int j) {
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+          const uint64_t da = smem_desc_sw128(smem + i * kQSubBytes + c * 16384);
+          const uint64_t db = smem_desc_sw128(ring + slot_of(j, c) * kSlotBytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16(tmem + i * 128, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
+        }
+        umma_commit(&s_full[i]);
+      };
+      auto issue_pv = [&](int i, int j) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint64_t db = smem_desc_mn_sw128(ring + slot_of(j, 3 + c) * kSlotBytes, 8192);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (c * 4 + k) * 8, db + 128 * k, kIdescPV,
+                        (j | c | k) != 0);
+        }
+        if (j + 1 == n_tiles[i]) umma_commit(&o_full[i]);
+      };
+      bool ok = mbar_wait(q_full, 0, a.status, s_abort) && wait_slots(0, 0, 3);
+      if (ok) {
+        tc_fence_after();
+        for (int i = 0; i < 2; ++i)
+          if (n_tiles[i] > 0) issue_qk(i, 0);
+        for (int c = 0; c < 3; ++c) umma_commit(&empty[slot_of(0, c)]);
+      }
+      for (int j = 0; j < n_max && ok; ++j) {
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (j < n_tiles[i]) {
+            if (!mbar_wait(&p_full[i], j & 1, a.status, s_abort)) { ok = false; break; }
+            if (i == 0 || n_tiles[0] <= j) {  // the first user of this tile's V
+              if (!wait_slots(j, 3, 5) || !mbar_wait(&v_ok[j & 1], (j >> 1) & 1, a.status, s_abort)) {
+                ok = false;
+                break;
+              }
+            }
+            tc_fence_after();
+            issue_pv(i, j);
+            if (i == 1 || n_tiles[1] <= j)
+              for (int c = 3; c < 5; ++c) umma_commit(&empty[slot_of(j, c)]);
+          }
+          if (j + 1 < n_tiles[i]) {
+            if (!wait_slots(j + 1, 0, 3)) { ok = false; break; }
+            tc_fence_after();
+            issue_qk(i, j + 1);
+            if (i == 1 || n_tiles[1] <= j + 1)
+              for (int c = 0; c < 3; ++c) umma_commit(&empty[slot_of(j + 1, c)]);
+          }
+        }
+      }
+      umma_commit(mma_done);  // every MMA issued here is done before TMEM is freed
+      mbar_wait(mma_done, 0, nullptr, nullptr);
+    }
+  } else if (warp >= 10) {
+    // ------------------------------------------------ V where a row may not see a key
+    // They pass every tile on (v_ok, two in turn: the ring holds no more than two tiles' V), so
+    // they see each phase of the ring's barriers.
+    const int vt = threadIdx.x - 320;  // 0 .. 63: a key row of each half
+    bool ok = true;
+    for (int j = 0; j < n_max && ok; ++j) {
+      bool wrote = false;
+#pragma unroll 1
+      for (int c = 3; c < 5; ++c) {
+        const int idx = 5 * j + c;
+        if (!mbar_wait(&full[idx % kPfSlots], (uint32_t)(idx / kPfSlots) & 1u, a.status, s_abort)) { ok = false; break; }
+        if (j < sure) continue;
+        uint8_t* base = ring + (idx % kPfSlots) * kSlotBytes + vt * 128;
+        const bool past = j * kPfTile + (c - 3) * 64 + vt >= nk;
+        uint32_t worst = 0;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            // any order of the row's eight 16-byte pieces will do; this one spreads the banks
+            uint4* p = reinterpret_cast<uint4*>(base + d * 8192 + ((x ^ (vt & 7)) << 4));
+            if (past) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              const uint4 v = *p;
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                worst = max(worst, max(w[y] & 0x7FFFu, (w[y] >> 16) & 0x7FFFu));
+              }
+            }
+          }
+        }
+        if (worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) *s_bad = 1;
+        wrote |= past;
+      }
+      if (wrote) fence_proxy_async_smem();
+      if (ok) mbar_arrive(&v_ok[j & 1]);
+    }
+  } else {
+    // ------------------------------------------------ softmax, one row per thread
+    const int sub = warp >> 2;
+    const int i_row = row0 + threadIdx.x;  // row of the request
+    const int limit = seen(i_row);
+    const int n_t = n_tiles[sub];
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // 32 lanes per warp
+    const uint32_t t_s = lane_base + sub * 128, t_o = lane_base + 256 + sub * 128;
+    float m_ref = -INFINITY, l = 0.f;  // in log2 units of the scaled scores
+    bool ok = true;
+    for (int j = 0; j < n_t; ++j) {
+      if (!mbar_wait(&s_full[sub], j & 1, a.status, s_abort)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t raw[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, raw[c]);
+      tmem_wait_ld();
+      if (a.neg) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) raw[c][x] ^= 0x80000000u;
+      }
+      const int vis = limit - j * kPfTile;  // keys of this tile that the row sees
+      if (__any_sync(0xffffffffu, vis < kPfTile)) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (c * 32 + x >= vis) raw[c][x] = 0xFF800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[c][x]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      const bool move = top > m_ref + kRescaleLog2 || m_ref == -INFINITY;
+      float f = 1.0f;
+      if (move) {
+        f = (m_ref == -INFINITY) ? 0.f : ex2(m_ref - top);
+        m_ref = top;
+        l *= f;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, move && f != 1.0f)) {
+        // this tile's scores are there, so the PV of the tile before it has finished
+        const float g = move ? f : 1.0f;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * g);
+          tmem_st32(t_o + c * 32, o);
+        }
+      }
+      const float base = m_ref == -INFINITY ? 0.f : m_ref;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const int e = c * 64 + 2 * x;
+          const float p0 = ex2(fmaf(__uint_as_float(raw[e >> 5][e & 31]), a.scale_log2, -base));
+          const float p1 = ex2(fmaf(__uint_as_float(raw[e >> 5][(e & 31) + 1]), a.scale_log2, -base));
+          sum[x & 1] += p0;
+          sum[2 + (x & 1)] += p1;
+          p[x] = ElemTraits<T>::pack2(p0, p1);
+        }
+        tmem_st32(t_s + c * 32, p);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[sub]);
+    }
+    if (n_t > 0 && ok) ok = mbar_wait(&o_full[sub], 0, a.status, s_abort);
+    tc_fence_after();
+    const bool live = i_row < nq;
+    const int64_t row = (q_lo + i_row) * a.heads + h;
+    if (*s_bad) {
+      if (ok)
+        for (int r = 0; r < 32; ++r) {
+          const int i = row0 + warp * 32 + r;
+          if (i < nq) prefill_row<T>(a, q_lo + i, h, k_lo, seen(i));
+        }
+    } else {
+      const bool some = l > 0.f || l != l;
+      const float inv = some ? 1.0f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (n_t > 0) {
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
+        }
+        if (live) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * kNopeDim + c * 32);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w[y] = some ? ElemTraits<T>::pack2(__uint_as_float(o[x * 8 + 2 * y]) * inv,
+                                                 __uint_as_float(o[x * 8 + 2 * y + 1]) * inv)
+                          : 0u;
+            dst[x] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (live && a.lse != nullptr) a.lse[row] = some ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+inline bool al16p(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T>
+cudaError_t launch_prefill(int dtype, PfArgs a, cudaStream_t st) {
+  CUtensorMap mq, mkv, mkr;
+  const uint64_t dq[3] = {(uint64_t)kQkDim, (uint64_t)a.tq, (uint64_t)a.heads};
+  const uint64_t sq[2] = {(uint64_t)a.q_st * 2, (uint64_t)a.q_sh * 2};
+  const uint64_t dkv[3] = {2 * (uint64_t)kNopeDim, (uint64_t)a.tk, (uint64_t)a.heads};
+  const uint64_t skv[2] = {(uint64_t)a.kv_st * 2, (uint64_t)a.kv_sh * 2};
+  const uint64_t dkr[2] = {(uint64_t)kRopeDim, (uint64_t)a.tk};
+  const uint64_t skr[1] = {(uint64_t)a.kr_st * 2};
+  if (!make_kmajor_map(&mq, dtype, a.q, 3, dq, sq, 64)) return cudaErrorInvalidValue;
+  if (a.tk > 0) {
+    if (!make_kmajor_map(&mkv, dtype, a.kv, 3, dkv, skv, 64) || !make_kmajor_map(&mkr, dtype, a.kr, 2, dkr, skr, 64))
+      return cudaErrorInvalidValue;
+  } else {
+    mkv = mkr = mq;  // no key tile is ever loaded
+  }
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(latent_prefill_kernel<T>), PfSmem::kBytes);
+  if (err != cudaSuccess) return err;
+  latent_prefill_kernel<T><<<(unsigned)((int64_t)a.units * a.heads), kPfThreads, PfSmem::kBytes, st>>>(mq, mkv, mkr, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
+                                  int64_t kv_stride_t, int64_t kv_stride_h, const void* k_rope, int64_t kr_stride_t,
+                                  const int32_t* cu_q, const int32_t* cu_k, int num_seqs, int64_t total_q,
+                                  int64_t total_k, int heads, float scale, int causal, void* out, float* lse,
+                                  int* status, void* stream) {
+  using namespace moe;
+  if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_FP16) return MOE_ERR_UNSUPPORTED;
+  if (num_seqs < 0 || total_q < 0 || total_k < 0 || heads <= 0) return MOE_ERR_INVALID_ARG;
+  if (total_q > INT32_MAX - 512 || total_k > INT32_MAX - 512 || heads > 65535 || num_seqs > 65535)
+    return MOE_ERR_BAD_SHAPE;
+  if (total_q == 0) return MOE_OK;
+  if (!q || !cu_q || !cu_k || !out || (total_k > 0 && (!kv || !k_rope))) return MOE_ERR_INVALID_ARG;
+  if (!al16p(q) || !al16p(kv) || !al16p(k_rope) || !al16p(out)) return MOE_ERR_INVALID_ARG;
+  // 16-byte TMA strides above zero; the stride of a dimension of one is not used
+  int64_t st[5] = {total_q > 1 ? q_stride_t : 8, heads > 1 ? q_stride_h : 8, total_k > 1 ? kv_stride_t : 8,
+                   heads > 1 ? kv_stride_h : 8, total_k > 1 ? kr_stride_t : 8};
+  for (int i = 0; i < 5; ++i)
+    if (st[i] <= 0 || st[i] % 8 || st[i] >= (int64_t)1 << 38) return MOE_ERR_BAD_SHAPE;
+  const int64_t units = total_q / 256 + num_seqs + 1;
+  if (units * heads > INT32_MAX) return MOE_ERR_BAD_SHAPE;
+  const int rc = moe_check_device();
+  if (rc != MOE_OK) return rc;
+  PfArgs a{q,     st[0], st[1], kv,     st[2],   st[3],   k_rope,  st[4],      cu_q, cu_k,
+           num_seqs, total_q, total_k, heads, (int)units, scale, 0.f, scale < 0.f, causal != 0, out,
+           lse,   status};
+  // flat softmax for a scale of zero: any scale this small gives scores of zero, and hidden places stay -inf
+  a.scale_log2 = scale == 0.f ? 1e-37f : (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = dtype == MOE_DTYPE_BF16 ? launch_prefill<__nv_bfloat16>(dtype, a, s)
+                                                  : launch_prefill<__half>(dtype, a, s);
+  return err == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+}
