@@ -34,4 +34,9 @@ __device__ __forceinline__ float ue8m0_value(uint32_t code) {
   return code == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(code << 23);
 }
 
+cudaError_t launch_latent_decode16(int dtype, const void* q, int num_seqs, int q_len, int heads, const void* cache,
+                                   int64_t num_pages, int page_size, const int32_t* table, int64_t ld_table,
+                                   int table_width, const int32_t* lens, float scale, void* out, float* lse,
+                                   void* workspace, int* status, cudaStream_t st);
+
 }  // namespace moe

@@ -113,11 +113,6 @@ inline bool al(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(
 }  // namespace
 }  // namespace moe
 
-extern "C" size_t moe_latent_decode_workspace_bytes(int64_t num_seqs, int q_len, int heads) {
-  if (num_seqs < 0 || q_len <= 0 || heads <= 0) return 0;
-  return 0;
-}
-
 extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int q_len, int heads, int cache_fmt,
                                  const void* cache, int64_t num_pages, int page_size, const int32_t* block_table,
                                  int64_t ld_table, int table_width, const int32_t* cache_lens, float scale, void* out,
@@ -131,6 +126,7 @@ extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int
       num_seqs > 65535 || (int64_t)table_width * page_size > INT32_MAX)
     return MOE_ERR_BAD_SHAPE;
   if (num_seqs == 0) return MOE_OK;
+  if (num_pages == 0) return MOE_ERR_INVALID_ARG;
   if (!q || !cache || !cache_lens || !out || (table_width > 0 && !block_table)) return MOE_ERR_INVALID_ARG;
   if (!al(q, 16) || !al(cache, 16) || !al(out, 16)) return MOE_ERR_INVALID_ARG;
   const size_t need = moe_latent_decode_workspace_bytes(num_seqs, q_len, heads);
@@ -145,9 +141,14 @@ extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int
   latent_decode_rows_kernel<T, F8><<<blocks, 32 * kRowsPerBlock, 0, st>>>(                                   \
       static_cast<const T*>(q), c, num_pages, page_size, block_table, ld_table, table_width, cache_lens, rows, q_len, \
       heads, scale, static_cast<T*>(out), lse, status)
-  if (cache_fmt == MOE_CACHE_E4M3) MOE_LD(__nv_bfloat16, true);
-  else if (dtype == MOE_DTYPE_BF16) MOE_LD(__nv_bfloat16, false);
-  else MOE_LD(__half, false);
+  if (cache_fmt == MOE_CACHE_E4M3) {
+    MOE_LD(__nv_bfloat16, true);
+  } else {
+    const cudaError_t e = launch_latent_decode16(dtype, q, (int)num_seqs, q_len, heads, cache, num_pages, page_size,
+                                                 block_table, ld_table, table_width, cache_lens, scale, out, lse,
+                                                 workspace, status, st);
+    return e == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+  }
 #undef MOE_LD
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }

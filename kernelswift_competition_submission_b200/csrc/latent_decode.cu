@@ -1,0 +1,841 @@
+// Latent attention over the paged cache, absorbed form, on the tensor cores (tcgen05 + TMEM + TMA).
+//
+//   s_j = scale q . [c_j, r_j],   o = sum_j softmax_j(s_j) c_j,   c_j 512 wide, r_j 64 wide
+// for every query row (request, draft token, head); all rows of a request share the cached rows, so
+// a tile is 128 rows (heads of one or several draft tokens) against 128 keys.
+//
+// A CTA pair (cta_group::2) takes a tile: each CTA holds 64 rows of Q, P and of O, whose 64 x 512 fp32
+// sums fill 256 of its 512 TMEM columns (a single CTA with 128 rows would need all of them and have
+// no place for the scores). For S = Q K^T each CTA supplies 64 of the 128 keys, for O += P V it
+// supplies half of V's columns, so a key's row crosses from L2 to shared memory twice per pair.
+//   warps 0-3  softmax: lane = row, warps 0-1 keys 0-63, warps 2-3 keys 64-127 of the tile; running
+//              maximum and sum, P into shared memory, O rescaled when the maximum has moved by 2^8
+//   warp 4     TMA producer: 16 KB slots ([64 keys][128 values]) in a ring of 8, in MMA order
+//   warp 5     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
+//              beside PV of j - 1 and QK of j + 1
+//
+// The (request, row tile, key tile) list is cut into equal runs, one per pair, by lengths read on
+// the device: no host copy of the lengths, every pair has the same work, whatever the mix. A
+// run that ends inside a request leaves its sum, maximum and unnormalised output in the workspace, and
+// a second kernel joins the pieces in key order (the same bits on every run).
+//
+// Masked places: scores are replaced before the maximum. V meets P = 0 in the MMA and 0 * NaN is
+// NaN, so in tiles that some row does not see whole the producer zeroes V past the length and looks
+// for non-finite values before the draft tokens; if there is one, the rows are computed again key by
+// key over visible keys.
+#include "latent.h"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+namespace moe {
+namespace {
+
+constexpr int kDcTile = 128;          // keys per tile, rows per pair
+constexpr int kDcRows = 64;           // rows per CTA
+constexpr int kDcSlots = 8;
+constexpr int kDcSlotBytes = 16384;   // [64 keys][128 values]
+constexpr int kDcMaxPairs = 80;
+constexpr int kDcThreads = 192;
+constexpr float kDcRescaleLog2 = 8.0f;
+
+struct DcSmem {
+  static constexpr int kRing = 9 * 8192;                      // after Q: nine [64 rows][64] chunks
+  static constexpr int kP = kRing + kDcSlots * kDcSlotBytes;  // two [64 rows][64 keys] chunks
+  static constexpr int kX = kP + 16384;                       // row maxima / sums of both key halves, two tiles
+  static constexpr int kBars = kX + 2 * 128 * 4;
+  // full[8], empty[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix
+  static constexpr int kNumBars = 2 * kDcSlots + 9;
+  static constexpr int kMisc = kBars + kNumBars * 8;
+  static constexpr int kBytes = kMisc + 64 + 1024;
+};
+
+struct DcArgs {
+  const void* q;
+  const uint8_t* cache;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;
+  int64_t num_pages;
+  int table_width, page_size, page_shift;
+  int num_seqs, n_q, heads, rows, row_tiles;
+  int pairs;
+  float scale, scale_log2;
+  int neg;
+  void* out;
+  float* lse;
+  float* part_o;    // [2 * pairs][part_rows][512]
+  float2* part_ml;  // [2 * pairs][part_rows]: maximum (log2 units) and sum
+  int part_rows;
+  int* status;
+};
+
+__device__ __forceinline__ float ex2d(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ int clamped_len(const DcArgs& a, int b) {
+  const int64_t cap = (int64_t)a.table_width << a.page_shift;
+  const int64_t n = __ldg(a.lens + b);
+  return (int)(n < 0 ? 0 : (n > cap ? cap : n));
+}
+__device__ __forceinline__ int len_tiles(int len) { return (len + kDcTile - 1) / kDcTile; }
+
+// Key tiles of all requests and row tiles, by one warp.
+__device__ __forceinline__ int64_t plan_total(const DcArgs& a) {
+  const int lane = threadIdx.x & 31;
+  int64_t n = 0;
+  for (int b = lane; b < a.num_seqs; b += 32) n += len_tiles(clamped_len(a, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * a.row_tiles;
+}
+__device__ __forceinline__ int64_t plan_chunk(const DcArgs& a, int64_t total) {
+  return max((int64_t)1, (total + a.pairs - 1) / a.pairs);
+}
+
+struct DcSeg {
+  int b, rt, k0, k1, n, len;  // key tiles [k0, k1) of n
+};
+// The segments of one pair's run, in order.
+struct DcIter {
+  int b;
+  int64_t off;   // tiles of request b before the next one
+  int64_t left;  // tiles of the run still to come
+  __device__ __forceinline__ bool next(const DcArgs& a, DcSeg& s) {
+    while (left > 0 && b < a.num_seqs) {
+      s.len = clamped_len(a, b);
+      s.n = len_tiles(s.len);
+      if (off >= (int64_t)s.n * a.row_tiles) {
+        off = 0;
+        ++b;
+        continue;
+      }
+      s.b = b;
+      s.rt = (int)(off / s.n);
+      s.k0 = (int)(off - (int64_t)s.rt * s.n);
+      s.k1 = (int)min((int64_t)s.n, s.k0 + left);
+      off += s.k1 - s.k0;
+      left -= s.k1 - s.k0;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Keys that row r of a request sees.
+__device__ __forceinline__ int row_seen(const DcArgs& a, int len, int r) {
+  return r >= a.rows ? 0 : max(0, len - a.n_q + 1 + r / a.heads);
+}
+
+// One row by a warp, key by key over [kb, ke): maximum and sum in natural units, output unnormalised;
+// lane l holds the elements 2 l, 2 l + 1 of every 64.
+template <typename T>
+__device__ __noinline__ void decode_row(const DcArgs& a, int b, int r, int kb, int ke, float& m, float& l,
+                                        float (&acc)[16]) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t* q =
+      reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.q) + ((int64_t)b * a.rows + r) * kRowDim);
+  float qv[18];
+#pragma unroll
+  for (int i = 0; i < 9; ++i) {
+    const float2 f = ElemTraits<T>::unpack2(__ldg(q + 32 * i + lane));
+    qv[2 * i] = f.x;
+    qv[2 * i + 1] = f.y;
+  }
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+  for (int j = kb; j < ke; ++j) {
+    const int64_t page = __ldg(a.table + b * a.ld_table + (j >> a.page_shift));
+    if (page < 0 || page >= a.num_pages) continue;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(
+        a.cache + (page * a.page_size + (j & (a.page_size - 1))) * (int64_t)(2 * kRowDim));
+    float k[18], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 9; ++i) {
+      const float2 f = ElemTraits<T>::unpack2(__ldg(src + 32 * i + lane));
+      k[2 * i] = f.x;
+      k[2 * i + 1] = f.y;
+    }
+#pragma unroll
+    for (int i = 0; i < 18; ++i) s = fmaf(qv[i], k[i], s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    s *= a.scale;
+    const float mn = fmaxf(m, s);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = expf(m - base), p = expf(s - base);
+    m = mn;
+    l = l * f + p;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = acc[i] * f + p * k[i];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDcThreads, 1)
+latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
+                     const __grid_constant__ DcArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + DcSmem::kRing;
+  uint8_t* s_p = smem + DcSmem::kP;
+  float* s_x = reinterpret_cast<float*>(smem + DcSmem::kX);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + DcSmem::kBars);
+  uint64_t* full = bars;                 // first CTA's: both CTAs' copies of a slot
+  uint64_t* empty = full + kDcSlots;     // each CTA's
+  uint64_t* q_full = empty + kDcSlots;   // first CTA's
+  uint64_t* q_free = q_full + 1;
+  uint64_t* s_full = q_free + 1;         // [2]
+  uint64_t* p_full = s_full + 2;         // first CTA's: eight softmax warps
+  uint64_t* pv_done = p_full + 1;
+  uint64_t* o_free = pv_done + 1;        // first CTA's: eight softmax warps
+  uint64_t* mma_done = o_free + 1;
+  uint64_t* fix = mma_done + 1;
+  int* misc = reinterpret_cast<int*>(smem + DcSmem::kMisc);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc);
+  volatile int* s_abort = misc + 1;
+  volatile int* s_bad = misc + 2;        // [2]: segment number + 1 whose V holds a non-finite value
+  volatile int* s_badpage = misc + 4;
+  int* s_plan = misc + 6;                // request, offset (2 words), tiles (2 words)
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = (int)cluster_id_x();
+
+  if (warp == 0) {
+    const int64_t total = plan_total(a), chunk = plan_chunk(a, total);
+    const int64_t start = min(total, pair * chunk), left = min(total, start + chunk) - start;
+    int64_t base = 0;
+    int found = a.num_seqs;
+    int64_t off = 0;
+    for (int b0 = 0; b0 < a.num_seqs && left > 0; b0 += 32) {
+      const int64_t n = b0 + lane < a.num_seqs ? (int64_t)len_tiles(clamped_len(a, b0 + lane)) * a.row_tiles : 0;
+      int64_t inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, start < base + inc);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        found = b0 + src;
+        off = start - base - __shfl_sync(0xffffffffu, inc - n, src);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) {
+      s_plan[0] = found;
+      *reinterpret_cast<int64_t*>(s_plan + 2) = off;
+      *reinterpret_cast<int64_t*>(s_plan + 4) = left;
+    }
+  }
+  if (threadIdx.x == 32) {
+    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
+    mbar_init(q_full, 2);
+    mbar_init(q_free, 1);
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(p_full, 8);
+    mbar_init(pv_done, 1);
+    mbar_init(o_free, 8);
+    mbar_init(mma_done, 1);
+    mbar_init(fix, 1);
+    *s_abort = 0;
+    s_bad[0] = s_bad[1] = 0;
+    *s_badpage = 0;
+    fence_mbar_init();
+  }
+  if (warp == 5) { tmem_alloc_pair(s_tmem, 512); tmem_relinquish_pair(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // barriers of both CTAs are ready
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  constexpr uint32_t kTmemS = 256;  // O: columns 0-127 and 128-255, S: 256-319 and 320-383
+  DcIter it{s_plan[0], *reinterpret_cast<int64_t*>(s_plan + 2), *reinterpret_cast<int64_t*>(s_plan + 4)};
+  DcSeg sg;
+
+  if (warp == 4) {
+    // ------------------------------------------------ TMA producer
+    if (lane == 0) { tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_c); }
+    const int br = min(a.page_size, 64), ppk = 64 / br;  // rows per copy, copies per 64 keys
+    int slot = 0, seg = 0;
+    uint32_t phase = 0, fix_phase = 0, issued = 0, issued_parity = 0;
+    bool ok = true;
+    auto wait_empty = [&]() {
+      bool r = true;
+      if (lane == 0) r = mbar_wait(&empty[slot], phase ^ 1, a.status, s_abort);
+      return __shfl_sync(0xffffffffu, (int)r, 0) != 0;
+    };
+    // pages of a tile: lane l (l < 8) that of keys 16 l .. 16 l + 15
+    auto pages_of = [&](const DcSeg& s, int j) {
+      const int64_t pi = ((int64_t)j * kDcTile + (lane & 7) * 16) >> a.page_shift;
+      return j < s.k1 && pi < a.table_width ? __ldg(a.table + s.b * a.ld_table + pi) : -1;
+    };
+    // [64 keys][nd * 64 values] of tile j from key half `half`, value d0, into the slot
+    auto copy = [&](int pages, int half, int j, int d0, int nd, uint64_t* local_bar) {
+      const int pr = lane % ppk, pd = lane / ppk;
+      const int key = half * 64 + pr * br;
+      const int page = __shfl_sync(0xffffffffu, pages, key >> 4);
+      if (pd < nd) {
+        uint8_t* dst = ring + slot * kDcSlotBytes + pd * 8192 + pr * br * 128;
+        const int row = (j * kDcTile + key) & (a.page_size - 1);
+        if (local_bar != nullptr) tma_load_3d(&map_c, local_bar, dst, d0 + pd * 64, row, page);
+        else tma_load_3d_pair(&map_c, mapa_shared(&full[slot], 0), dst, d0 + pd * 64, row, page);
+      }
+    };
+    auto announce = [&](uint32_t bytes) {  // one arrival per CTA; the first one also expects both CTAs' bytes
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
+        else mbar_arrive_cluster(mapa_shared(&full[slot], 0));
+      }
+      __syncwarp();
+    };
+    auto step = [&]() {
+      issued |= 1u << slot;
+      issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
+      if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+    };
+    auto load_k = [&](int pages, int j) {
+      for (int c = 0; c < 5; ++c) {
+        if (!wait_empty()) return false;
+        const int nd = c < 4 ? 2 : 1;
+        announce((uint32_t)nd * 8192u);
+        copy(pages, (int)rank, j, c * 128, nd, nullptr);
+        step();
+      }
+      return true;
+    };
+    auto load_v = [&](const DcSeg& s, int pages, int j) {
+      // slot order: value block 0 keys 0-63, 64-127, value block 1 keys 0-63, 64-127
+      const int sure = max(0, s.len - a.n_q + 1);  // keys that every row sees
+      if ((j + 1) * kDcTile <= sure) {
+        for (int c = 0; c < 4; ++c) {
+          if (!wait_empty()) return false;
+          announce(kDcSlotBytes);
+          copy(pages, c & 1, j, (c >> 1) * 256 + (int)rank * 128, 2, nullptr);
+          step();
+        }
+        return true;
+      }
+      // some row does not see all of this tile: bring V in on this CTA's own barrier, zero the rows
+      // past the length, look at the rows some query may not see, then hand the slots over
+      const int slot0 = slot;
+      const uint32_t phase0 = phase;
+      for (int c = 0; c < 4; ++c) {
+        if (!wait_empty()) return false;
+        if (c == 0 && lane == 0) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
+        __syncwarp();
+        copy(pages, c & 1, j, (c >> 1) * 256 + (int)rank * 128, 2, fix);
+        step();
+      }
+      bool r = true;
+      if (lane == 0) r = mbar_wait(fix, fix_phase, a.status, s_abort);
+      fix_phase ^= 1;
+      if (!__shfl_sync(0xffffffffu, (int)r, 0)) return false;
+      uint32_t worst = 0;
+      for (int c = 0; c < 4; ++c) {
+        uint8_t* base = ring + ((slot0 + c) % kDcSlots) * kDcSlotBytes;
+        const int key0 = j * kDcTile + (c & 1) * 64;
+        for (int v = max(0, sure - key0) * 16 + lane; v < 64 * 16; v += 32) {  // 16-byte pieces of rows >= sure
+          const int row = v >> 4;
+          uint4* p = reinterpret_cast<uint4*>(base + ((v >> 3) & 1) * 8192 + row * 128 + (v & 7) * 16);
+          if (key0 + row >= s.len) {
+            *p = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            const uint4 x = *p;
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) worst = max(worst, max(w[y] & 0x7FFFu, (w[y] >> 16) & 0x7FFFu));
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) && lane < 2) {
+        const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      const int slot1 = slot;
+      const uint32_t phase1 = phase;
+      slot = slot0;
+      phase = phase0;
+      for (int c = 0; c < 4; ++c) {
+        announce(0);
+        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+      }
+      slot = slot1;
+      phase = phase1;
+      return true;
+    };
+    while (ok && it.next(a, sg)) {
+      if (seg > 0) {  // the query rows of the segment before are no longer read
+        bool r = true;
+        if (lane == 0) r = mbar_wait(q_free, (seg - 1) & 1, a.status, s_abort);
+        if (!__shfl_sync(0xffffffffu, (int)r, 0)) { ok = false; break; }
+      }
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
+        else mbar_arrive_cluster(mapa_shared(q_full, 0));
+      }
+      __syncwarp();
+      if (lane < 9)
+        tma_load_3d_pair(&map_q, mapa_shared(q_full, 0), smem + lane * 8192, lane * 64,
+                         sg.rt * kDcTile + (int)rank * kDcRows, sg.b);
+      int pg0 = pages_of(sg, sg.k0), pg1 = pages_of(sg, sg.k0 + 1), pg2 = pages_of(sg, sg.k0 + 2);
+      ok = load_k(pg0, sg.k0);
+      if (ok && sg.k0 + 1 < sg.k1) ok = load_k(pg1, sg.k0 + 1);
+      for (int j = sg.k0; j < sg.k1 && ok; ++j) {
+        const int pg3 = pages_of(sg, j + 3);
+        ok = load_v(sg, pg0, j);
+        if (ok && j + 2 < sg.k1) ok = load_k(pg2, j + 2);
+        pg0 = pg1;
+        pg1 = pg2;
+        pg2 = pg3;
+      }
+      ++seg;
+    }
+    if (!ok && rank == 0 && lane == 0) {  // wait (bounded) for copies in flight before the pair may leave
+      for (int s = 0; s < kDcSlots; ++s)
+        if ((issued >> s) & 1u) mbar_wait<true>(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+    }
+  } else if (warp == 5) {
+    if (rank == 0 && lane == 0) {
+      // ------------------------------------------------ MMA issuer
+      constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
+      constexpr uint32_t kIdescPV = idesc_f16(128, 256, ElemTraits<T>::kFmt) | kIdescBMnMajor;
+      int slot = 0, seg = 0, g = 0;  // g: tiles of the run so far
+      uint32_t phase = 0;
+      bool ok = true;
+      auto take = [&]() {
+        const bool r = mbar_wait<true>(&full[slot], phase, a.status, s_abort);
+        tc_fence_after();
+        return r;
+      };
+      auto give = [&]() {
+        umma_commit_pair_multicast(&empty[slot], 0x3);
+        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+      };
+      auto issue_qk = [&](int tile) {
+        const uint32_t d = tmem + kTmemS + (tile & 1) * 64;
+        for (int c = 0; c < 5; ++c) {
+          if (!take()) return false;
+          const int nk = c < 4 ? 8 : 4;
+          for (int k = 0; k < nk; ++k) {
+            const uint64_t da = smem_desc_sw128(smem + (2 * c + (k >> 2)) * 8192) + 2 * (k & 3);
+            const uint64_t db = smem_desc_sw128(ring + slot * kDcSlotBytes + (k >> 2) * 8192) + 2 * (k & 3);
+            umma_f16_pair(d, da, db, kIdescQK, (c | k) != 0);
+          }
+          give();
+        }
+        umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
+        return true;
+      };
+      while (ok && it.next(a, sg)) {
+        const int nt = sg.k1 - sg.k0;
+        if (!mbar_wait<true>(q_full, seg & 1, a.status, s_abort)) { ok = false; break; }
+        ok = issue_qk(g) && (nt < 2 || issue_qk(g + 1));
+        if (nt <= 2) umma_commit_pair_multicast(q_free, 0x3);
+        for (int j = 0; j < nt && ok; ++j) {
+          if (j == 0 && seg > 0 && !mbar_wait<true>(o_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
+          if (!mbar_wait<true>(p_full, (g + j) & 1, a.status, s_abort)) { ok = false; break; }
+          for (int c = 0; c < 4; ++c) {
+            if (!take()) { ok = false; break; }
+            const uint64_t db = smem_desc_mn_sw128(ring + slot * kDcSlotBytes, 8192);
+            for (int k = 0; k < 4; ++k)
+              umma_f16_pair(tmem + (c >> 1) * 128, smem_desc_sw128(s_p + (c & 1) * 8192) + 2 * k, db + 128 * k, kIdescPV,
+                            (j | (c & 1) | k) != 0);
+            give();
+          }
+          if (!ok) break;
+          umma_commit_pair_multicast(pv_done, 0x3);
+          if (j + 2 < nt) {
+            ok = issue_qk(g + j + 2);
+            if (j + 3 == nt) umma_commit_pair_multicast(q_free, 0x3);
+          }
+        }
+        g += nt;
+        ++seg;
+      }
+      umma_commit_pair(mma_done);  // every MMA issued here is done before TMEM is freed
+      mbar_wait(mma_done, 0, nullptr, nullptr);
+    }
+  } else {
+    // ------------------------------------------------ softmax
+    const int half = warp >> 1;                  // key half of S, value half of O
+    const int r = (warp & 1) * 32 + lane;        // row of this CTA
+    const uint32_t lane_base = tmem + ((uint32_t)warp << 21);
+    int seg = 0, g = 0;
+    bool ok = true;
+    while (ok && it.next(a, sg)) {
+      const int row = sg.rt * kDcTile + (int)rank * kDcRows + r;  // row of the request
+      const int limit = row_seen(a, sg.len, row);
+      float m_ref = -INFINITY, l = 0.f;
+      // the segment's pages: a bad one hides its keys (their V arrives as zeros)
+      {
+        if (threadIdx.x == 0) {
+          const int n = __ldg(a.lens + sg.b);
+          if (n != sg.len) record_status(a.status, MOE_ERR_INVALID_ARG);
+        }
+        const int first = (int)(((int64_t)sg.k0 * kDcTile) >> a.page_shift);
+        const int last = (int)((min((int64_t)sg.k1 * kDcTile, (int64_t)sg.len) - 1) >> a.page_shift);
+        bool bad = false;
+        for (int p = first + (int)threadIdx.x; p <= last; p += 128) {
+          const int v = __ldg(a.table + sg.b * a.ld_table + p);
+          bad |= v < 0 || v >= a.num_pages;
+        }
+        if (bad) { record_status(a.status, MOE_ERR_INVALID_ARG); *s_badpage = seg + 1; }
+        named_bar_sync(1, 128);
+      }
+      const bool bad_page = *s_badpage == seg + 1;
+      for (int j = sg.k0; j < sg.k1; ++j, ++g) {
+        // a wait that gave up is carried to the next barrier of the four warps, so that all leave together
+        ok = mbar_wait<true>(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
+        tc_fence_after();
+        uint32_t raw[2][32];
+        tmem_ld32(lane_base + kTmemS + (g & 1) * 64, raw[0]);
+        tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + 32, raw[1]);
+        tmem_wait_ld();
+        if (a.neg) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x) raw[c][x] ^= 0x80000000u;
+        }
+        const int key0 = j * kDcTile + half * 64;
+        const int vis = limit - key0;
+        if (__any_sync(0xffffffffu, vis < 64)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if (c * 32 + x >= vis) raw[c][x] = 0xFF800000u;
+        }
+        if (bad_page) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int64_t pi = ((int64_t)key0 + u * 16) >> a.page_shift;
+            const int v = pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
+            if (v < 0 || v >= a.num_pages) {
+#pragma unroll
+              for (int x = 0; x < 16; ++x) raw[u >> 1][(u & 1) * 16 + x] = 0xFF800000u;
+            }
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[c][x]));
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // the row's other 64 keys are with the thread 64 further on
+        float* x = s_x + (g & 1) * 128;
+        x[threadIdx.x] = top;
+        ok = named_bar_and(1, 128, ok);
+        if (!ok) break;
+        top = fmaxf(top, x[threadIdx.x ^ 64]) * a.scale_log2;
+        const bool move = top > m_ref + kDcRescaleLog2 || m_ref == -INFINITY;
+        float f = 1.0f;
+        if (move) {
+          f = (m_ref == -INFINITY) ? 0.f : ex2d(m_ref - top);
+          m_ref = top;
+          l *= f;
+        }
+        const float base = m_ref == -INFINITY ? 0.f : m_ref;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t p[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = ex2d(fmaf(__uint_as_float(raw[e >> 4][(2 * e) & 31]), a.scale_log2, -base));
+          const float p1 = ex2d(fmaf(__uint_as_float(raw[e >> 4][((2 * e) & 31) + 1]), a.scale_log2, -base));
+          sum[e & 1] += p0;
+          sum[2 + (e & 1)] += p1;
+          p[e] = ElemTraits<T>::pack2(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (j > sg.k0) {  // PV of the tile before: its P is read, its O is written
+          ok = mbar_wait<true>(pv_done, (g - 1) & 1, a.status, s_abort) && ok;
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, move && f != 1.0f)) {
+            const float w = move ? f : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[32];
+              tmem_ld32(lane_base + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w);
+              tmem_st32(lane_base + c * 32, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        uint8_t* dst = s_p + half * 8192 + r * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) =
+              make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(p_full, 0));
+      }
+      ok = ok && mbar_wait<true>(pv_done, (g - 1) & 1, a.status, s_abort);
+      tc_fence_after();
+      // ---------------------------------------------- end of the segment
+      ok = named_bar_and(1, 128, ok);  // the maxima of the last tile are read
+      if (!ok) break;
+      s_x[threadIdx.x] = l;
+      named_bar_sync(1, 128);
+      l += s_x[threadIdx.x ^ 64];
+      const bool whole = sg.k0 == 0 && sg.k1 == sg.n;
+      const int64_t pslot = 2 * pair + (sg.k0 == 0 ? 1 : 0);
+      const bool live = row < a.rows;
+      if (s_bad[seg & 1] == seg + 1) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(o_free, 0));
+        for (int rr = warp; rr < kDcRows; rr += 4) {
+          const int rw = sg.rt * kDcTile + (int)rank * kDcRows + rr;
+          if (rw >= a.rows) break;
+          float m, ls, acc[16];
+          decode_row<T>(a, sg.b, rw, sg.k0 * kDcTile, min(row_seen(a, sg.len, rw), sg.k1 * kDcTile), m, ls, acc);
+          const bool some = ls > 0.f || ls != ls;
+          if (whole) {
+            const int64_t o = (int64_t)sg.b * a.rows + rw;
+            const float inv = some ? 1.f / ls : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + o * kLatDim)[32 * i + lane] =
+                  ElemTraits<T>::pack2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+            if (a.lse != nullptr && lane == 0) a.lse[o] = some ? m + logf(ls) : -INFINITY;
+          } else {
+            const int64_t o = pslot * a.part_rows + (int)rank * kDcRows + rr;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<float2*>(a.part_o + o * kLatDim)[32 * i + lane] = make_float2(acc[2 * i], acc[2 * i + 1]);
+            if (lane == 0) a.part_ml[o] = make_float2(m * 1.4426950408889634f, ls);
+          }
+        }
+      } else {
+        const bool some = l > 0.f || l != l;
+        const float inv = some ? 1.0f / l : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {  // TMEM columns 32 c: values 256 (c / 4) + 128 half + 32 (c % 4)
+          uint32_t o[32];
+          tmem_ld32(lane_base + c * 32, o);
+          tmem_wait_ld();
+          const int d = (c >> 2) * 256 + half * 128 + (c & 3) * 32;
+          if (live) {
+            if (whole) {
+              uint4* dst =
+                  reinterpret_cast<uint4*>(static_cast<T*>(a.out) + ((int64_t)sg.b * a.rows + row) * kLatDim + d);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t w[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  w[y] = some ? ElemTraits<T>::pack2(__uint_as_float(o[e * 8 + 2 * y]) * inv,
+                                                     __uint_as_float(o[e * 8 + 2 * y + 1]) * inv)
+                              : 0u;
+                dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(a.part_o + (pslot * a.part_rows + (int)rank * kDcRows + r) * kLatDim + d);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            }
+          }
+        }
+        if (live && half == 0) {
+          if (!whole) a.part_ml[pslot * a.part_rows + (int)rank * kDcRows + r] = make_float2(m_ref, l);
+          else if (a.lse != nullptr)
+            a.lse[(int64_t)sg.b * a.rows + row] = some ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(o_free, 0));
+      }
+      named_bar_sync(1, 128);  // s_x is free again
+      ++seg;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while its peer may use its barriers, shared memory or TMEM
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc_pair(tmem, 512);
+}
+
+// Joins the pieces of requests that several pairs worked on, and writes the rows of empty ones: one
+// warp per row, pieces in key order.
+template <typename T>
+__global__ void __launch_bounds__(128)
+latent_decode_join_kernel(const __grid_constant__ DcArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (int64_t)a.num_seqs * a.rows) return;
+  const int b = (int)(row / a.rows), r = (int)(row - (int64_t)b * a.rows), rt = r / kDcTile;
+  int64_t total = 0, before = 0;
+  for (int i = lane; i < a.num_seqs; i += 32) {
+    const int n = len_tiles(clamped_len(a, i));
+    total += n;
+    before += i < b ? n : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  const int64_t chunk = plan_chunk(a, total * a.row_tiles);
+  const int n = len_tiles(clamped_len(a, b));
+  T* out = static_cast<T*>(a.out) + row * kLatDim;
+  if (n == 0) {
+    for (int i = lane; i < kLatDim / 8; i += 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (lane == 0) {
+      if (a.lse != nullptr) a.lse[row] = -INFINITY;
+      if (__ldg(a.lens + b) != 0) record_status(a.status, MOE_ERR_INVALID_ARG);
+    }
+    return;
+  }
+  const int64_t g0 = before * a.row_tiles + (int64_t)rt * n;
+  const int p0 = (int)(g0 / chunk), p1 = (int)((g0 + n - 1) / chunk);
+  if (p0 == p1) return;  // one pair had all of it
+  auto place = [&](int p) { return (int64_t)(2 * p + (p == p0 ? 1 : 0)) * a.part_rows + (r - rt * kDcTile); };
+  float m = -INFINITY;
+  for (int p = p0 + lane; p <= p1; p += 32) m = fmaxf(m, a.part_ml[place(p)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = p0; p <= p1; ++p) {
+    const int64_t s = place(p);
+    const float2 ml = a.part_ml[s];
+    if (ml.y == 0.f) continue;  // saw nothing; a NaN sum goes on
+    const float w = ex2d(ml.x - base);
+    l += w * ml.y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(a.part_o + s * kLatDim)[32 * i + lane];
+      acc[i].x += w * v.x;
+      acc[i].y += w * v.y;
+      acc[i].z += w * v.z;
+      acc[i].w += w * v.w;
+    }
+  }
+  const bool some = l > 0.f || l != l;
+  const float inv = some ? 1.f / l : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<uint2*>(out)[32 * i + lane] =
+        make_uint2(ElemTraits<T>::pack2(acc[i].x * inv, acc[i].y * inv), ElemTraits<T>::pack2(acc[i].z * inv, acc[i].w * inv));
+  if (lane == 0 && a.lse != nullptr) a.lse[row] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+}
+
+constexpr int kMaxDev = 64;
+
+// CTA pairs that can be resident at once (a pair needs two SMs of one cluster); asked once per device.
+template <typename K>
+cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
+  static int cache[kMaxDev];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev >= 0 && dev < kMaxDev && cache[dev] > 0) {
+    *pairs = cache[dev];
+    return cudaSuccess;
+  }
+  cfg.gridDim = dim3((unsigned)num_sms() / 2 * 2, 1, 1);
+  int n = 0;
+  err = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+  if (err != cudaSuccess) return err;
+  if (n <= 0) return cudaErrorInvalidConfiguration;
+  *pairs = std::min(n, kDcMaxPairs);
+  if (dev >= 0 && dev < kMaxDev) cache[dev] = *pairs;
+  return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
+  CUtensorMap mq, mc;
+  const uint64_t dq[3] = {(uint64_t)kRowDim, (uint64_t)a.rows, (uint64_t)a.num_seqs};
+  const uint64_t sq[2] = {2 * (uint64_t)kRowDim, 2 * (uint64_t)kRowDim * (uint64_t)a.rows};
+  const uint64_t dc[3] = {(uint64_t)kRowDim, (uint64_t)a.page_size, (uint64_t)std::max<int64_t>(a.num_pages, 1)};
+  const uint64_t sc[2] = {2 * (uint64_t)kRowDim, 2 * (uint64_t)kRowDim * (uint64_t)a.page_size};
+  if (!make_kmajor_map(&mq, dtype, a.q, 3, dq, sq, 64) ||
+      !make_kmajor_map(&mc, dtype, a.cache, 3, dc, sc, (uint32_t)std::min(a.page_size, 64)))
+    return cudaErrorInvalidValue;
+  auto kern = latent_decode_kernel<T>;
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(kern), DcSmem::kBytes);
+  if (err != cudaSuccess) return err;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kDcThreads, 1, 1);
+  cfg.dynamicSmemBytes = DcSmem::kBytes;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if ((err = resident_pairs(kern, cfg, &a.pairs)) != cudaSuccess) return err;
+  cfg.gridDim = dim3(2 * (unsigned)a.pairs, 1, 1);
+  if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, a)) != cudaSuccess) return err;
+  latent_decode_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.num_seqs * a.rows, 4), 128, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_latent_decode16(int dtype, const void* q, int num_seqs, int q_len, int heads, const void* cache,
+                                   int64_t num_pages, int page_size, const int32_t* table, int64_t ld_table,
+                                   int table_width, const int32_t* lens, float scale, void* out, float* lse,
+                                   void* workspace, int* status, cudaStream_t st) {
+  DcArgs a{};
+  a.q = q;
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.table = table;
+  a.ld_table = ld_table;
+  a.lens = lens;
+  a.num_pages = num_pages;
+  a.table_width = table_width;
+  a.page_size = page_size;
+  a.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  a.num_seqs = num_seqs;
+  a.n_q = q_len;
+  a.heads = heads;
+  a.rows = q_len * heads;
+  a.row_tiles = (int)ceil_div(a.rows, kDcTile);
+  a.scale = scale;
+  // flat softmax for a scale of zero: any scale this small gives scores of zero, and hidden places stay -inf
+  a.scale_log2 = scale == 0.f ? 1e-37f : (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  a.neg = scale < 0.f;
+  a.out = out;
+  a.lse = lse;
+  a.part_rows = std::min(a.rows, kDcTile);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * (size_t)kDcMaxPairs * a.part_rows * kLatDim);
+  a.status = status;
+  return dtype == MOE_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(dtype, a, st) : launch_decode<__half>(dtype, a, st);
+}
+
+}  // namespace moe
+
+extern "C" size_t moe_latent_decode_workspace_bytes(int64_t num_seqs, int q_len, int heads) {
+  if (num_seqs < 0 || q_len <= 0 || heads <= 0) return 0;
+  const size_t rows = (size_t)std::min<int64_t>((int64_t)q_len * heads, moe::kDcTile);
+  return 2 * (size_t)moe::kDcMaxPairs * rows * (moe::kLatDim * 4 + 8);
+}
