@@ -45,8 +45,8 @@ struct DcSmem {
   static constexpr int kP = kRing + kDcSlots * kDcSlotBytes;  // two [64 rows][64 keys] chunks
   static constexpr int kX = kP + 16384;                       // row maxima / sums of both key halves, two tiles
   static constexpr int kBars = kX + 2 * 128 * 4;
-  // full[8], empty[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix
-  static constexpr int kNumBars = 2 * kDcSlots + 9;
+  // full[8], empty[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix, v_fixed
+  static constexpr int kNumBars = 2 * kDcSlots + 10;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kBytes = kMisc + 64 + 1024;
 };
@@ -197,6 +197,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint64_t* o_free = pv_done + 1;        // first CTA's: eight softmax warps
   uint64_t* mma_done = o_free + 1;
   uint64_t* fix = mma_done + 1;
+  uint64_t* v_fixed = fix + 1;           // first CTA's: the other CTA has looked at its V
   int* misc = reinterpret_cast<int*>(smem + DcSmem::kMisc);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc);
   volatile int* s_abort = misc + 1;
@@ -238,8 +239,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], 2); mbar_init(&empty[s], 1); }
-    mbar_init(q_full, 2);
+    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
@@ -248,6 +249,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     mbar_init(o_free, 8);
     mbar_init(mma_done, 1);
     mbar_init(fix, 1);
+    mbar_init(v_fixed, 1);
     *s_abort = 0;
     s_bad[0] = s_bad[1] = 0;
     *s_badpage = 0;
@@ -266,7 +268,11 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   if (warp == 4) {
     // ------------------------------------------------ TMA producer
     if (lane == 0) { tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_c); }
-    const int br = min(a.page_size, 64), ppk = 64 / br;  // rows per copy, copies per 64 keys
+    // one copy per slot when a page holds 64 keys, else one per page and 64 values, a lane each
+    const int br = min(a.page_size, 64), ppk = 64 / br;
+    const int pr = br == 64 ? 0 : lane % ppk, pd = br == 64 ? 2 * lane : lane / ppk;
+    const uint32_t dst_off = (uint32_t)(pd * 8192 + pr * br * 128);
+    const uint32_t full0 = mapa_shared(full, 0);
     int slot = 0, seg = 0;
     uint32_t phase = 0, fix_phase = 0, issued = 0, issued_parity = 0;
     bool ok = true;
@@ -280,24 +286,21 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const int64_t pi = ((int64_t)j * kDcTile + (lane & 7) * 16) >> a.page_shift;
       return j < s.k1 && pi < a.table_width ? __ldg(a.table + s.b * a.ld_table + pi) : -1;
     };
-    // [64 keys][nd * 64 values] of tile j from key half `half`, value d0, into the slot
-    auto copy = [&](int pages, int half, int j, int d0, int nd, uint64_t* local_bar) {
-      const int pr = lane % ppk, pd = lane / ppk;
+    // 64 keys (key half `half`) of tile j, 64-value chunks ch and ch + 1, into the slot. Chunk 9 does not
+    // exist and reads as zeros, so the rotary chunk's slot counts the same bytes.
+    auto copy = [&](int pages, int half, int j, int ch, uint64_t* local_bar) {
       const int key = half * 64 + pr * br;
       const int page = __shfl_sync(0xffffffffu, pages, key >> 4);
-      if (pd < nd) {
-        uint8_t* dst = ring + slot * kDcSlotBytes + pd * 8192 + pr * br * 128;
+      if (pd < 2) {
+        uint8_t* dst = ring + slot * kDcSlotBytes + dst_off;
         const int row = (j * kDcTile + key) & (a.page_size - 1);
-        if (local_bar != nullptr) tma_load_3d(&map_c, local_bar, dst, d0 + pd * 64, row, page);
-        else tma_load_3d_pair(&map_c, mapa_shared(&full[slot], 0), dst, d0 + pd * 64, row, page);
+        if (local_bar != nullptr) tma_load_4d(&map_c, local_bar, dst, 0, row, ch + pd, page);
+        else tma_load_4d_pair(&map_c, full0 + slot * 8, dst, 0, row, ch + pd, page);
       }
     };
-    auto announce = [&](uint32_t bytes) {  // one arrival per CTA; the first one also expects both CTAs' bytes
-      if (lane == 0) {
-        if (rank == 0) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
-        else mbar_arrive_cluster(mapa_shared(&full[slot], 0));
-      }
-      __syncwarp();
+    // the first CTA's arrival expects both CTAs' bytes; the other's may be there before it
+    auto announce = [&](uint32_t bytes) {
+      if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
     };
     auto step = [&]() {
       issued |= 1u << slot;
@@ -307,9 +310,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     auto load_k = [&](int pages, int j) {
       for (int c = 0; c < 5; ++c) {
         if (!wait_empty()) return false;
-        const int nd = c < 4 ? 2 : 1;
-        announce((uint32_t)nd * 8192u);
-        copy(pages, (int)rank, j, c * 128, nd, nullptr);
+        announce(kDcSlotBytes);
+        copy(pages, (int)rank, j, c * 2, nullptr);
         step();
       }
       return true;
@@ -321,7 +323,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         for (int c = 0; c < 4; ++c) {
           if (!wait_empty()) return false;
           announce(kDcSlotBytes);
-          copy(pages, c & 1, j, (c >> 1) * 256 + (int)rank * 128, 2, nullptr);
+          copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, nullptr);
           step();
         }
         return true;
@@ -334,7 +336,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (!wait_empty()) return false;
         if (c == 0 && lane == 0) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
         __syncwarp();
-        copy(pages, c & 1, j, (c >> 1) * 256 + (int)rank * 128, 2, fix);
+        copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, fix);
         step();
       }
       bool r = true;
@@ -364,6 +366,10 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       fence_proxy_async_smem();
       __syncwarp();
+      if (rank != 0) {
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
+        return true;
+      }
       const int slot1 = slot;
       const uint32_t phase1 = phase;
       slot = slot0;
@@ -384,12 +390,9 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       if (lane == 0) {
         if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
-        else mbar_arrive_cluster(mapa_shared(q_full, 0));
+        tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
       }
       __syncwarp();
-      if (lane < 9)
-        tma_load_3d_pair(&map_q, mapa_shared(q_full, 0), smem + lane * 8192, lane * 64,
-                         sg.rt * kDcTile + (int)rank * kDcRows, sg.b);
       int pg0 = pages_of(sg, sg.k0), pg1 = pages_of(sg, sg.k0 + 1), pg2 = pages_of(sg, sg.k0 + 2);
       ok = load_k(pg0, sg.k0);
       if (ok && sg.k0 + 1 < sg.k1) ok = load_k(pg1, sg.k0 + 1);
@@ -405,18 +408,18 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
     if (!ok && rank == 0 && lane == 0) {  // wait (bounded) for copies in flight before the pair may leave
       for (int s = 0; s < kDcSlots; ++s)
-        if ((issued >> s) & 1u) mbar_wait<true>(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+        if ((issued >> s) & 1u) mbar_wait(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
     }
   } else if (warp == 5) {
     if (rank == 0 && lane == 0) {
       // ------------------------------------------------ MMA issuer
       constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
       constexpr uint32_t kIdescPV = idesc_f16(128, 256, ElemTraits<T>::kFmt) | kIdescBMnMajor;
-      int slot = 0, seg = 0, g = 0;  // g: tiles of the run so far
+      int slot = 0, seg = 0, g = 0, n_fixed = 0;  // g: tiles of the run so far
       uint32_t phase = 0;
       bool ok = true;
       auto take = [&]() {
-        const bool r = mbar_wait<true>(&full[slot], phase, a.status, s_abort);
+        const bool r = mbar_wait(&full[slot], phase, a.status, s_abort);
         tc_fence_after();
         return r;
       };
@@ -424,15 +427,18 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         umma_commit_pair_multicast(&empty[slot], 0x3);
         if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
       };
+      const uint64_t dq0 = smem_desc_sw128(smem), dk0 = smem_desc_sw128(ring), dp0 = smem_desc_sw128(s_p);
+      const uint64_t dv0 = smem_desc_mn_sw128(ring, 8192);
       auto issue_qk = [&](int tile) {
         const uint32_t d = tmem + kTmemS + (tile & 1) * 64;
+#pragma unroll
         for (int c = 0; c < 5; ++c) {
           if (!take()) return false;
-          const int nk = c < 4 ? 8 : 4;
-          for (int k = 0; k < nk; ++k) {
-            const uint64_t da = smem_desc_sw128(smem + (2 * c + (k >> 2)) * 8192) + 2 * (k & 3);
-            const uint64_t db = smem_desc_sw128(ring + slot * kDcSlotBytes + (k >> 2) * 8192) + 2 * (k & 3);
-            umma_f16_pair(d, da, db, kIdescQK, (c | k) != 0);
+          const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < (c < 4 ? 8 : 4); ++k) {
+            const uint32_t step = (k >> 2) * (8192 >> 4) + 2 * (k & 3);
+            umma_f16_pair(d, dq0 + c * (16384 >> 4) + step, db + step, kIdescQK, (c | k) != 0);
           }
           give();
         }
@@ -441,17 +447,24 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       };
       while (ok && it.next(a, sg)) {
         const int nt = sg.k1 - sg.k0;
-        if (!mbar_wait<true>(q_full, seg & 1, a.status, s_abort)) { ok = false; break; }
+        if (!mbar_wait(q_full, seg & 1, a.status, s_abort)) { ok = false; break; }
         ok = issue_qk(g) && (nt < 2 || issue_qk(g + 1));
         if (nt <= 2) umma_commit_pair_multicast(q_free, 0x3);
         for (int j = 0; j < nt && ok; ++j) {
-          if (j == 0 && seg > 0 && !mbar_wait<true>(o_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
-          if (!mbar_wait<true>(p_full, (g + j) & 1, a.status, s_abort)) { ok = false; break; }
+          if (j == 0 && seg > 0 && !mbar_wait(o_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
+          if (!mbar_wait(p_full, (g + j) & 1, a.status, s_abort)) { ok = false; break; }
+          const int sure = max(0, sg.len - a.n_q + 1);
+          if ((sg.k0 + j + 1) * kDcTile > sure) {
+            if (!mbar_wait(v_fixed, n_fixed & 1, a.status, s_abort)) { ok = false; break; }
+            ++n_fixed;
+          }
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
             if (!take()) { ok = false; break; }
-            const uint64_t db = smem_desc_mn_sw128(ring + slot * kDcSlotBytes, 8192);
+            const uint64_t db = dv0 + (uint32_t)slot * (kDcSlotBytes >> 4);
+#pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16_pair(tmem + (c >> 1) * 128, smem_desc_sw128(s_p + (c & 1) * 8192) + 2 * k, db + 128 * k, kIdescPV,
+              umma_f16_pair(tmem + (c >> 1) * 128, dp0 + (c & 1) * (8192 >> 4) + 2 * k, db + 128 * k, kIdescPV,
                             (j | (c & 1) | k) != 0);
             give();
           }
@@ -498,7 +511,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const bool bad_page = *s_badpage == seg + 1;
       for (int j = sg.k0; j < sg.k1; ++j, ++g) {
         // a wait that gave up is carried to the next barrier of the four warps, so that all leave together
-        ok = mbar_wait<true>(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
+        ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
         tc_fence_after();
         uint32_t raw[2][32];
         tmem_ld32(lane_base + kTmemS + (g & 1) * 64, raw[0]);
@@ -562,7 +575,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (j > sg.k0) {  // PV of the tile before: its P is read, its O is written
-          ok = mbar_wait<true>(pv_done, (g - 1) & 1, a.status, s_abort) && ok;
+          ok = mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort) && ok;
           tc_fence_after();
           if (__any_sync(0xffffffffu, move && f != 1.0f)) {
             const float w = move ? f : 1.0f;
@@ -588,7 +601,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(p_full, 0));
       }
-      ok = ok && mbar_wait<true>(pv_done, (g - 1) & 1, a.status, s_abort);
+      ok = ok && mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort);
       tc_fence_after();
       // ---------------------------------------------- end of the segment
       ok = named_bar_and(1, 128, ok);  // the maxima of the last tile are read
@@ -770,12 +783,14 @@ cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
 template <typename T>
 cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   CUtensorMap mq, mc;
-  const uint64_t dq[3] = {(uint64_t)kRowDim, (uint64_t)a.rows, (uint64_t)a.num_seqs};
-  const uint64_t sq[2] = {2 * (uint64_t)kRowDim, 2 * (uint64_t)kRowDim * (uint64_t)a.rows};
-  const uint64_t dc[3] = {(uint64_t)kRowDim, (uint64_t)a.page_size, (uint64_t)std::max<int64_t>(a.num_pages, 1)};
-  const uint64_t sc[2] = {2 * (uint64_t)kRowDim, 2 * (uint64_t)kRowDim * (uint64_t)a.page_size};
-  if (!make_kmajor_map(&mq, dtype, a.q, 3, dq, sq, 64) ||
-      !make_kmajor_map(&mc, dtype, a.cache, 3, dc, sc, (uint32_t)std::min(a.page_size, 64)))
+  const uint64_t row = 2 * kRowDim;
+  const uint64_t dq[4] = {64, (uint64_t)a.rows, kRowDim / 64, (uint64_t)a.num_seqs};
+  const uint64_t sq[3] = {row, 128, row * (uint64_t)a.rows};
+  const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
+  const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
+  const uint32_t box_rows = (uint32_t)std::min(a.page_size, 64);
+  if (!make_chunks_map(&mq, dtype, a.q, dq, sq, kDcRows, kRowDim / 64) ||
+      !make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1))
     return cudaErrorInvalidValue;
   auto kern = latent_decode_kernel<T>;
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(kern), DcSmem::kBytes);

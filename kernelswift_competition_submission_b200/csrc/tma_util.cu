@@ -33,12 +33,13 @@ EncodeTiledFn get_encode_fn() {
 struct MapKey {
   int device, kind, dtype, rank;
   const void* base;
-  uint64_t dims[3], strides[2];
-  uint32_t box_rows;
+  uint64_t dims[4], strides[3];
+  uint32_t box_rows, box_outer;
   bool operator==(const MapKey& o) const {
     return device == o.device && kind == o.kind && dtype == o.dtype && rank == o.rank && base == o.base &&
-           dims[0] == o.dims[0] && dims[1] == o.dims[1] && dims[2] == o.dims[2] && strides[0] == o.strides[0] &&
-           strides[1] == o.strides[1] && box_rows == o.box_rows;
+           dims[0] == o.dims[0] && dims[1] == o.dims[1] && dims[2] == o.dims[2] && dims[3] == o.dims[3] &&
+           strides[0] == o.strides[0] && strides[1] == o.strides[1] && strides[2] == o.strides[2] &&
+           box_rows == o.box_rows && box_outer == o.box_outer;
   }
 };
 
@@ -60,8 +61,8 @@ MapKey map_key(int kind, int dtype, const void* base, int rank, const uint64_t* 
   k.dtype = dtype;
   k.rank = rank;
   k.base = base;
-  for (int i = 0; i < rank && i < 3; ++i) k.dims[i] = dims[i];
-  for (int i = 0; i < rank - 1 && i < 2; ++i) k.strides[i] = strides[i];
+  for (int i = 0; i < rank && i < 4; ++i) k.dims[i] = dims[i];
+  for (int i = 0; i < rank - 1 && i < 3; ++i) k.strides[i] = strides[i];
   k.box_rows = box_rows;
   return k;
 }
@@ -88,7 +89,7 @@ void cache_store(const MapKey& k, const CUtensorMap& m) {
   g_maps.stamp[victim] = ++g_maps.clock;
 }
 
-enum { kMapKMajor16 = 0, kMapFp8 = 1, kMapF32Rows = 2 };
+enum { kMapKMajor16 = 0, kMapFp8 = 1, kMapF32Rows = 2, kMapChunks16 = 3 };
 
 }  // namespace
 
@@ -107,6 +108,29 @@ bool make_kmajor_map(CUtensorMap* m, int dtype, const void* base, int rank, cons
   const CUtensorMapDataType dt =
       dtype == MOE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (enc(m, dt, rank, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
+      CUDA_SUCCESS)
+    return false;
+  cache_store(key, *m);
+  return true;
+}
+
+// 16-bit map of rank 4 whose box is `box_chunks` blocks of [box_rows][64 elements], each with the
+// 128-byte swizzle: dims {64, rows, 64-element chunks, outer}.
+bool make_chunks_map(CUtensorMap* m, int dtype, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
+                     uint32_t box_rows, uint32_t box_chunks) {
+  MapKey key = map_key(kMapChunks16, dtype, base, 4, dims, strides_bytes, box_rows);
+  key.box_outer = box_chunks;
+  if (cache_lookup(key, m)) return true;
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return false;
+  cuuint64_t gdim[4], gstr[3];
+  cuuint32_t box[4] = {64, box_rows, box_chunks, 1}, estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) gdim[i] = dims[i];
+  for (int i = 0; i < 3; ++i) gstr[i] = strides_bytes[i];
+  const CUtensorMapDataType dt =
+      dtype == MOE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (enc(m, dt, 4, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
       CUDA_SUCCESS)
     return false;
