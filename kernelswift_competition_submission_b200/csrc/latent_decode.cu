@@ -99,6 +99,15 @@ __device__ __forceinline__ int64_t plan_chunk(const DcArgs& a, int64_t total) {
 
 struct DcSeg {
   int b, rt, k0, k1, n, len;  // key tiles [k0, k1) of n
+  // the same values, known to be equal over the warp
+  __device__ __forceinline__ void uniform() {
+    b = __shfl_sync(0xffffffffu, b, 0);
+    rt = __shfl_sync(0xffffffffu, rt, 0);
+    k0 = __shfl_sync(0xffffffffu, k0, 0);
+    k1 = __shfl_sync(0xffffffffu, k1, 0);
+    n = __shfl_sync(0xffffffffu, n, 0);
+    len = __shfl_sync(0xffffffffu, len, 0);
+  }
 };
 // The segments of one pair's run, in order.
 struct DcIter {
@@ -205,7 +214,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   volatile int* s_badpage = misc + 4;
   int* s_plan = misc + 6;                // request, offset (2 words), tiles (2 words)
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = (int)cluster_id_x();
 
@@ -268,39 +277,44 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   if (warp == 4) {
     // ------------------------------------------------ TMA producer
     if (lane == 0) { tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_c); }
-    // one copy per slot when a page holds 64 keys, else one per page and 64 values, a lane each
+    const bool one = elect_one();
+    // one copy per slot when a page holds 64 keys, else one per page and 64 values
     const int br = min(a.page_size, 64), ppk = 64 / br;
-    const int pr = br == 64 ? 0 : lane % ppk, pd = br == 64 ? 2 * lane : lane / ppk;
-    const uint32_t dst_off = (uint32_t)(pd * 8192 + pr * br * 128);
     const uint32_t full0 = mapa_shared(full, 0);
     int slot = 0, seg = 0;
     uint32_t phase = 0, fix_phase = 0, issued = 0, issued_parity = 0;
     bool ok = true;
-    auto wait_empty = [&]() {
-      bool r = true;
-      if (lane == 0) r = mbar_wait(&empty[slot], phase ^ 1, a.status, s_abort);
-      return __shfl_sync(0xffffffffu, (int)r, 0) != 0;
-    };
+    auto wait_empty = [&]() { return mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort); };
     // pages of a tile: lane l (l < 8) that of keys 16 l .. 16 l + 15
     auto pages_of = [&](const DcSeg& s, int j) {
       const int64_t pi = ((int64_t)j * kDcTile + (lane & 7) * 16) >> a.page_shift;
       return j < s.k1 && pi < a.table_width ? __ldg(a.table + s.b * a.ld_table + pi) : -1;
     };
+    auto copy_one = [&](int dst_off, int row, int ch, int page, bool local) {
+      uint8_t* dst = ring + slot * kDcSlotBytes + dst_off;
+      if (one) {
+        if (local) tma_load_4d(&map_c, fix, dst, 0, row, ch, page);
+        else tma_load_4d_pair(&map_c, full0 + slot * 8, dst, 0, row, ch, page);
+      }
+      __syncwarp();
+    };
     // 64 keys (key half `half`) of tile j, 64-value chunks ch and ch + 1, into the slot. Chunk 9 does not
-    // exist and reads as zeros, so the rotary chunk's slot counts the same bytes.
-    auto copy = [&](int pages, int half, int j, int ch, uint64_t* local_bar) {
-      const int key = half * 64 + pr * br;
-      const int page = __shfl_sync(0xffffffffu, pages, key >> 4);
-      if (pd < 2) {
-        uint8_t* dst = ring + slot * kDcSlotBytes + dst_off;
-        const int row = (j * kDcTile + key) & (a.page_size - 1);
-        if (local_bar != nullptr) tma_load_4d(&map_c, local_bar, dst, 0, row, ch + pd, page);
-        else tma_load_4d_pair(&map_c, full0 + slot * 8, dst, 0, row, ch + pd, page);
+    // exist and reads as zeros, so the rotary chunk's slot counts the same bytes. `local`: counted on
+    // this CTA's `fix`, else on the first CTA's `full`.
+    auto copy = [&](int pages, int half, int j, int ch, bool local) {
+      if (br == 64) {
+        copy_one(0, (j * kDcTile + half * 64) & (a.page_size - 1), ch, __shfl_sync(0xffffffffu, pages, half * 4), local);
+      } else {
+        for (int i = 0; i < ppk; ++i) {
+          const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
+          for (int d = 0; d < 2; ++d) copy_one(d * 8192 + i * br * 128, 0, ch + d, page, local);
+        }
       }
     };
     // the first CTA's arrival expects both CTAs' bytes; the other's may be there before it
     auto announce = [&](uint32_t bytes) {
-      if (rank == 0 && lane == 0) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
+      if (rank == 0 && one) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
+      __syncwarp();
     };
     auto step = [&]() {
       issued |= 1u << slot;
@@ -311,7 +325,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       for (int c = 0; c < 5; ++c) {
         if (!wait_empty()) return false;
         announce(kDcSlotBytes);
-        copy(pages, (int)rank, j, c * 2, nullptr);
+        copy(pages, (int)rank, j, c * 2, false);
         step();
       }
       return true;
@@ -323,7 +337,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         for (int c = 0; c < 4; ++c) {
           if (!wait_empty()) return false;
           announce(kDcSlotBytes);
-          copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, nullptr);
+          copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, false);
           step();
         }
         return true;
@@ -334,15 +348,13 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const uint32_t phase0 = phase;
       for (int c = 0; c < 4; ++c) {
         if (!wait_empty()) return false;
-        if (c == 0 && lane == 0) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
+        if (c == 0 && one) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
         __syncwarp();
-        copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, fix);
+        copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, true);
         step();
       }
-      bool r = true;
-      if (lane == 0) r = mbar_wait(fix, fix_phase, a.status, s_abort);
+      if (!mbar_wait_warp(fix, fix_phase, a.status, s_abort)) return false;
       fix_phase ^= 1;
-      if (!__shfl_sync(0xffffffffu, (int)r, 0)) return false;
       uint32_t worst = 0;
       for (int c = 0; c < 4; ++c) {
         uint8_t* base = ring + ((slot0 + c) % kDcSlots) * kDcSlotBytes;
@@ -367,7 +379,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       fence_proxy_async_smem();
       __syncwarp();
       if (rank != 0) {
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
+        if (one) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
+        __syncwarp();
         return true;
       }
       const int slot1 = slot;
@@ -383,12 +396,10 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       return true;
     };
     while (ok && it.next(a, sg)) {
-      if (seg > 0) {  // the query rows of the segment before are no longer read
-        bool r = true;
-        if (lane == 0) r = mbar_wait(q_free, (seg - 1) & 1, a.status, s_abort);
-        if (!__shfl_sync(0xffffffffu, (int)r, 0)) { ok = false; break; }
-      }
-      if (lane == 0) {
+      sg.uniform();
+      // the query rows of the segment before are no longer read
+      if (seg > 0 && !mbar_wait_warp(q_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
+      if (one) {
         if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
         tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
       }
@@ -406,80 +417,93 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       ++seg;
     }
-    if (!ok && rank == 0 && lane == 0) {  // wait (bounded) for copies in flight before the pair may leave
+    if (!ok && rank == 0) {  // wait (bounded) for copies in flight before the pair may leave
       for (int s = 0; s < kDcSlots; ++s)
-        if ((issued >> s) & 1u) mbar_wait(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+        if ((issued >> s) & 1u) mbar_wait_warp(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
     }
   } else if (warp == 5) {
-    if (rank == 0 && lane == 0) {
-      // ------------------------------------------------ MMA issuer
+    if (rank == 0) {
+      // ------------------------------------------------ MMA issuer: the warp converged, one lane issues
       constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
       constexpr uint32_t kIdescPV = idesc_f16(128, 256, ElemTraits<T>::kFmt) | kIdescBMnMajor;
+      const bool one = elect_one();
       int slot = 0, seg = 0, g = 0, n_fixed = 0;  // g: tiles of the run so far
       uint32_t phase = 0;
       bool ok = true;
-      auto take = [&]() {
-        const bool r = mbar_wait(&full[slot], phase, a.status, s_abort);
-        tc_fence_after();
-        return r;
-      };
-      auto give = [&]() {
-        umma_commit_pair_multicast(&empty[slot], 0x3);
-        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
-      };
       const uint64_t dq0 = smem_desc_sw128(smem), dk0 = smem_desc_sw128(ring), dp0 = smem_desc_sw128(s_p);
       const uint64_t dv0 = smem_desc_mn_sw128(ring, 8192);
+      auto take = [&]() {
+        ok = mbar_wait_warp(&full[slot], phase, a.status, s_abort) && ok;
+        tc_fence_after();
+      };
+      auto next_slot = [&]() {
+        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+      };
       auto issue_qk = [&](int tile) {
         const uint32_t d = tmem + kTmemS + (tile & 1) * 64;
 #pragma unroll
         for (int c = 0; c < 5; ++c) {
-          if (!take()) return false;
-          const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4);
+          take();
+          if (one) {
+            const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < (c < 4 ? 8 : 4); ++k) {
-            const uint32_t step = (k >> 2) * (8192 >> 4) + 2 * (k & 3);
-            umma_f16_pair(d, dq0 + c * (16384 >> 4) + step, db + step, kIdescQK, (c | k) != 0);
+            for (int k = 0; k < (c < 4 ? 8 : 4); ++k) {
+              const uint32_t step = (k >> 2) * (8192 >> 4) + 2 * (k & 3);
+              umma_f16_pair(d, dq0 + c * (16384 >> 4) + step, db + step, kIdescQK, (c | k) != 0);
+            }
+            umma_commit_pair_multicast(&empty[slot], 0x3);
+            if (c == 4) umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
           }
-          give();
+          __syncwarp();
+          next_slot();
         }
-        umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
-        return true;
       };
+      auto free_q = [&]() {
+        if (one) umma_commit_pair_multicast(q_free, 0x3);
+        __syncwarp();
+      };
+      // a wait that gave up ends the loops at the next tile; until then the MMAs run on what is there
       while (ok && it.next(a, sg)) {
+        sg.uniform();
         const int nt = sg.k1 - sg.k0;
-        if (!mbar_wait(q_full, seg & 1, a.status, s_abort)) { ok = false; break; }
-        ok = issue_qk(g) && (nt < 2 || issue_qk(g + 1));
-        if (nt <= 2) umma_commit_pair_multicast(q_free, 0x3);
+        const int sure = max(0, sg.len - a.n_q + 1);
+        ok = mbar_wait_warp(q_full, seg & 1, a.status, s_abort);
+        issue_qk(g);
+        if (nt > 1) issue_qk(g + 1);
+        if (nt <= 2) free_q();
         for (int j = 0; j < nt && ok; ++j) {
-          if (j == 0 && seg > 0 && !mbar_wait(o_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
-          if (!mbar_wait(p_full, (g + j) & 1, a.status, s_abort)) { ok = false; break; }
-          const int sure = max(0, sg.len - a.n_q + 1);
+          if (j == 0 && seg > 0) ok = mbar_wait_warp(o_free, (seg - 1) & 1, a.status, s_abort) && ok;
           if ((sg.k0 + j + 1) * kDcTile > sure) {
-            if (!mbar_wait(v_fixed, n_fixed & 1, a.status, s_abort)) { ok = false; break; }
+            ok = mbar_wait_warp(v_fixed, n_fixed & 1, a.status, s_abort) && ok;
             ++n_fixed;
           }
+          ok = mbar_wait_warp(p_full, (g + j) & 1, a.status, s_abort) && ok;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (!take()) { ok = false; break; }
-            const uint64_t db = dv0 + (uint32_t)slot * (kDcSlotBytes >> 4);
+            take();
+            if (one) {
+              const uint64_t db = dv0 + (uint32_t)slot * (kDcSlotBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_pair(tmem + (c >> 1) * 128, dp0 + (c & 1) * (8192 >> 4) + 2 * k, db + 128 * k, kIdescPV,
-                            (j | (c & 1) | k) != 0);
-            give();
+              for (int k = 0; k < 4; ++k)
+                umma_f16_pair(tmem + (c >> 1) * 128, dp0 + (c & 1) * (8192 >> 4) + 2 * k, db + 128 * k, kIdescPV,
+                              (j | (c & 1) | k) != 0);
+              umma_commit_pair_multicast(&empty[slot], 0x3);
+              if (c == 3) umma_commit_pair_multicast(pv_done, 0x3);
+            }
+            __syncwarp();
+            next_slot();
           }
-          if (!ok) break;
-          umma_commit_pair_multicast(pv_done, 0x3);
           if (j + 2 < nt) {
-            ok = issue_qk(g + j + 2);
-            if (j + 3 == nt) umma_commit_pair_multicast(q_free, 0x3);
+            issue_qk(g + j + 2);
+            if (j + 3 == nt) free_q();
           }
         }
         g += nt;
         ++seg;
       }
-      umma_commit_pair(mma_done);  // every MMA issued here is done before TMEM is freed
-      mbar_wait(mma_done, 0, nullptr, nullptr);
+      if (one) umma_commit_pair(mma_done);  // every MMA issued here is done before TMEM is freed
+      __syncwarp();
+      mbar_wait_warp(mma_done, 0, nullptr, nullptr);
     }
   } else {
     // ------------------------------------------------ softmax

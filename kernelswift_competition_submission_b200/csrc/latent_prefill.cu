@@ -119,7 +119,8 @@ __device__ __noinline__ void prefill_row(const PfArgs& a, int64_t t, int h, int6
 template <typename T>
 __global__ void __launch_bounds__(kPfThreads, 1)
 latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
-                      const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ PfArgs a) {
+                      const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ CUtensorMap map_v,
+                      const __grid_constant__ PfArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + PfSmem::kRing;
@@ -138,7 +139,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   volatile int* s_bad = misc + 2;
   int* s_unit = misc + 4;  // request, tile
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x / a.units;
   const int unit = a.units - 1 - (blockIdx.x - h * a.units);
 
@@ -228,115 +229,133 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const uint32_t tmem = *s_tmem;
 
   if (warp == 8) {
-    if (lane == 0) {
-      // ------------------------------------------------ TMA producer
-      tma_prefetch_desc(&map_q);
+    // ------------------------------------------------ TMA producer: the warp converged, one lane issues
+    const bool one = elect_one();
+    if (one) {
       tma_prefetch_desc(&map_kv);
       tma_prefetch_desc(&map_kr);
+      tma_prefetch_desc(&map_v);
       mbar_arrive_expect_tx(q_full, 2 * kQSubBytes);
       for (int i = 0; i < 2; ++i)
         for (int c = 0; c < 3; ++c)
-          for (int r = 0; r < 2; ++r)
-            tma_load_3d(&map_q, q_full, smem + i * kQSubBytes + c * 16384 + r * 8192, c * 64,
-                        (int)q_lo + row0 + i * kPfTile + r * 64, h);
-      int slot = 0;
-      uint32_t phase = 0, issued = 0, issued_parity = 0;
-      bool ok = true;
-      for (int j = 0; j < n_max && ok; ++j) {
-        const int kt = (int)k_lo + j * kPfTile;
-        for (int c = 0; c < 5; ++c) {
-          if (!mbar_wait(&empty[slot], phase ^ 1, a.status, s_abort)) { ok = false; break; }
-          uint8_t* dst = ring + slot * kSlotBytes;
-          mbar_arrive_expect_tx(&full[slot], kSlotBytes);
-          if (c < 2) {
-            tma_load_3d(&map_kv, &full[slot], dst, c * 64, kt, h);
-            tma_load_3d(&map_kv, &full[slot], dst + 8192, c * 64, kt + 64, h);
-          } else if (c == 2) {
-            tma_load_2d(&map_kr, &full[slot], dst, 0, kt);
-            tma_load_2d(&map_kr, &full[slot], dst + 8192, 0, kt + 64);
-          } else {
-            tma_load_3d(&map_kv, &full[slot], dst, kNopeDim, kt + (c - 3) * 64, h);
-            tma_load_3d(&map_kv, &full[slot], dst + 8192, kNopeDim + 64, kt + (c - 3) * 64, h);
+          tma_load_3d(&map_q, q_full, smem + i * kQSubBytes + c * 16384, c * 64, (int)q_lo + row0 + i * kPfTile, h);
+    }
+    __syncwarp();
+    int slot = 0;
+    uint32_t phase = 0, issued = 0, issued_parity = 0;
+    bool ok = true;
+    for (int j = 0; j < n_max && ok; ++j) {
+      const int kt = (int)k_lo + j * kPfTile;
+#pragma unroll
+      for (int c = 0; c < 5; ++c) {
+        if (ok) {
+          ok = mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort);
+          if (ok) {
+            uint8_t* dst = ring + slot * kSlotBytes;
+            if (one) {
+              mbar_arrive_expect_tx(&full[slot], kSlotBytes);
+              if (c < 2) tma_load_3d(&map_kv, &full[slot], dst, c * 64, kt, h);
+              else if (c == 2) tma_load_2d(&map_kr, &full[slot], dst, 0, kt);
+              else tma_load_4d(&map_v, &full[slot], dst, 0, kt + (c - 3) * 64, 2, h);
+            }
+            __syncwarp();
+            issued |= 1u << slot;
+            issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
+            if (++slot == kPfSlots) { slot = 0; phase ^= 1; }
           }
-          issued |= 1u << slot;
-          issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
-          if (++slot == kPfSlots) { slot = 0; phase ^= 1; }
         }
       }
-      if (!ok) {  // wait (bounded) for the copies in flight before the CTA may leave
-        mbar_wait(q_full, 0, nullptr, nullptr);
-        for (int s = 0; s < kPfSlots; ++s)
-          if ((issued >> s) & 1u) mbar_wait(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
-      }
+    }
+    if (!ok) {  // wait (bounded) for the copies in flight before the CTA may leave
+      mbar_wait_warp(q_full, 0, nullptr, nullptr);
+      for (int s = 0; s < kPfSlots; ++s)
+        if ((issued >> s) & 1u) mbar_wait_warp(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
     }
   } else if (warp == 9) {
-    if (lane == 0) {
-      // ------------------------------------------------ MMA issuer
-      constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
-      constexpr uint32_t kIdescPV = idesc_f16(128, 128, ElemTraits<T>::kFmt) | kIdescBMnMajor;
-      // ring position of tile j's K (0..2) and V (3, 4)
-      auto slot_of = [&](int j, int c) { return (5 * j + c) % kPfSlots; };
-      auto phase_of = [&](int j, int c) { return (uint32_t)((5 * j + c) / kPfSlots) & 1u; };
-      auto wait_slots = [&](int j, int c0, int c1) {
-        for (int c = c0; c < c1; ++c)
-          if (!mbar_wait(&full[slot_of(j, c)], phase_of(j, c), a.status, s_abort)) return false;
-        return true;
-      };
-      auto issue_qk = [&](int i, int j) {
+    // ------------------------------------------------ MMA issuer: the warp converged, one lane issues
+    constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
+    constexpr uint32_t kIdescPV = idesc_f16(128, 128, ElemTraits<T>::kFmt) | kIdescBMnMajor;
+    const bool one = elect_one();
+    const uint64_t dq0 = smem_desc_sw128(smem), dk0 = smem_desc_sw128(ring), dv0 = smem_desc_mn_sw128(ring, 8192);
+    bool ok = true;
+    int kslot = 0, vslot = 3;  // ring position of the tile's K (three slots) and V (two)
+    uint32_t kphase = 0, vphase = 0;
+    auto at = [](int s) { return s >= kPfSlots ? s - kPfSlots : s; };
+    auto wait_slots = [&](int s0, int n, uint32_t ph) {
+      for (int c = 0; c < n; ++c)
+        ok = mbar_wait_warp(&full[at(s0 + c)], s0 + c >= kPfSlots ? ph ^ 1 : ph, a.status, s_abort) && ok;
+      tc_fence_after();
+    };
+    // S of subtile i from the K at kslot; `last`: no later user of this K
+    auto issue_qk = [&](int i, bool last) {
+      if (one) {
 #pragma unroll
         for (int c = 0; c < 3; ++c) {
-          const uint64_t da = smem_desc_sw128(smem + i * kQSubBytes + c * 16384);
-          const uint64_t db = smem_desc_sw128(ring + slot_of(j, c) * kSlotBytes);
+          const uint64_t da = dq0 + i * (kQSubBytes >> 4) + c * (16384 >> 4);
+          const uint64_t db = dk0 + (uint32_t)at(kslot + c) * (kSlotBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_f16(tmem + i * 128, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
         }
         umma_commit(&s_full[i]);
-      };
-      auto issue_pv = [&](int i, int j) {
+        if (last)
+          for (int c = 0; c < 3; ++c) umma_commit(&empty[at(kslot + c)]);
+      }
+      __syncwarp();
+    };
+    auto issue_pv = [&](int i, bool first, bool fin, bool last) {
+      if (one) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const uint64_t db = smem_desc_mn_sw128(ring + slot_of(j, 3 + c) * kSlotBytes, 8192);
+          const uint64_t db = dv0 + (uint32_t)at(vslot + c) * (kSlotBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (c * 4 + k) * 8, db + 128 * k, kIdescPV,
-                        (j | c | k) != 0);
+                        !first || (c | k) != 0);
         }
-        if (j + 1 == n_tiles[i]) umma_commit(&o_full[i]);
-      };
-      bool ok = mbar_wait(q_full, 0, a.status, s_abort) && wait_slots(0, 0, 3);
-      if (ok) {
-        tc_fence_after();
-        for (int i = 0; i < 2; ++i)
-          if (n_tiles[i] > 0) issue_qk(i, 0);
-        for (int c = 0; c < 3; ++c) umma_commit(&empty[slot_of(0, c)]);
+        if (fin) umma_commit(&o_full[i]);
+        if (last)
+          for (int c = 0; c < 2; ++c) umma_commit(&empty[at(vslot + c)]);
       }
-      for (int j = 0; j < n_max && ok; ++j) {
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (j < n_tiles[i]) {
-            if (!mbar_wait(&p_full[i], j & 1, a.status, s_abort)) { ok = false; break; }
-            if (i == 0 || n_tiles[0] <= j) {  // the first user of this tile's V
-              if (!wait_slots(j, 3, 5) || !mbar_wait(&v_ok[j & 1], (j >> 1) & 1, a.status, s_abort)) {
-                ok = false;
-                break;
-              }
-            }
-            tc_fence_after();
-            issue_pv(i, j);
-            if (i == 1 || n_tiles[1] <= j)
-              for (int c = 3; c < 5; ++c) umma_commit(&empty[slot_of(j, c)]);
+      __syncwarp();
+    };
+    auto forward = [&](int& s, uint32_t& ph) {
+      s += 5;
+      if (s >= kPfSlots) { s -= kPfSlots; ph ^= 1; }
+    };
+    // a wait that gave up ends the loop at the next tile; until then the MMAs run on what is there
+    ok = mbar_wait_warp(q_full, 0, a.status, s_abort);
+    wait_slots(0, 3, 0);
+    if (n_tiles[0] > 0) issue_qk(0, n_tiles[1] == 0);
+    if (n_tiles[1] > 0) issue_qk(1, true);
+    forward(kslot, kphase);
+    for (int j = 0; j < n_max && ok; ++j) {
+      bool v_here = false, k_here = false;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (j < n_tiles[i]) {
+          if (!v_here) {
+            wait_slots(vslot, 2, vphase);
+            ok = mbar_wait_warp(&v_ok[j & 1], (j >> 1) & 1, a.status, s_abort) && ok;
+            v_here = true;
           }
-          if (j + 1 < n_tiles[i]) {
-            if (!wait_slots(j + 1, 0, 3)) { ok = false; break; }
-            tc_fence_after();
-            issue_qk(i, j + 1);
-            if (i == 1 || n_tiles[1] <= j + 1)
-              for (int c = 0; c < 3; ++c) umma_commit(&empty[slot_of(j + 1, c)]);
+          ok = mbar_wait_warp(&p_full[i], j & 1, a.status, s_abort) && ok;
+          tc_fence_after();
+          issue_pv(i, j == 0, j + 1 == n_tiles[i], i == 1 || n_tiles[1] <= j);
+        }
+        if (j + 1 < n_tiles[i]) {
+          if (!k_here) {
+            wait_slots(kslot, 3, kphase);
+            k_here = true;
           }
+          issue_qk(i, i == 1 || n_tiles[1] <= j + 1);
         }
       }
-      umma_commit(mma_done);  // every MMA issued here is done before TMEM is freed
-      mbar_wait(mma_done, 0, nullptr, nullptr);
+      forward(vslot, vphase);
+      forward(kslot, kphase);
     }
+    if (one) umma_commit(mma_done);  // every MMA issued here is done before TMEM is freed
+    __syncwarp();
+    mbar_wait_warp(mma_done, 0, nullptr, nullptr);
   } else if (warp >= 10) {
     // ------------------------------------------------ V where a row may not see a key
     // They pass every tile on (v_ok, two in turn: the ring holds no more than two tiles' V), so
@@ -505,23 +524,28 @@ inline bool al16p(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u)
 
 template <typename T>
 cudaError_t launch_prefill(int dtype, PfArgs a, cudaStream_t st) {
-  CUtensorMap mq, mkv, mkr;
+  CUtensorMap mq, mkv, mkr, mv;
   const uint64_t dq[3] = {(uint64_t)kQkDim, (uint64_t)a.tq, (uint64_t)a.heads};
   const uint64_t sq[2] = {(uint64_t)a.q_st * 2, (uint64_t)a.q_sh * 2};
   const uint64_t dkv[3] = {2 * (uint64_t)kNopeDim, (uint64_t)a.tk, (uint64_t)a.heads};
   const uint64_t skv[2] = {(uint64_t)a.kv_st * 2, (uint64_t)a.kv_sh * 2};
   const uint64_t dkr[2] = {(uint64_t)kRopeDim, (uint64_t)a.tk};
   const uint64_t skr[1] = {(uint64_t)a.kr_st * 2};
-  if (!make_kmajor_map(&mq, dtype, a.q, 3, dq, sq, 64)) return cudaErrorInvalidValue;
+  if (!make_kmajor_map(&mq, dtype, a.q, 3, dq, sq, kPfTile)) return cudaErrorInvalidValue;
   if (a.tk > 0) {
-    if (!make_kmajor_map(&mkv, dtype, a.kv, 3, dkv, skv, 64) || !make_kmajor_map(&mkr, dtype, a.kr, 2, dkr, skr, 64))
+    // V: both 64-value chunks of 64 keys in one box
+    const uint64_t dv[4] = {64, (uint64_t)a.tk, 4, (uint64_t)a.heads};
+    const uint64_t sv[3] = {(uint64_t)a.kv_st * 2, 128, (uint64_t)a.kv_sh * 2};
+    if (!make_kmajor_map(&mkv, dtype, a.kv, 3, dkv, skv, kPfTile) ||
+        !make_kmajor_map(&mkr, dtype, a.kr, 2, dkr, skr, kPfTile) || !make_chunks_map(&mv, dtype, a.kv, dv, sv, 64, 2))
       return cudaErrorInvalidValue;
   } else {
-    mkv = mkr = mq;  // no key tile is ever loaded
+    mkv = mkr = mv = mq;  // no key tile is ever loaded
   }
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(latent_prefill_kernel<T>), PfSmem::kBytes);
   if (err != cudaSuccess) return err;
-  latent_prefill_kernel<T><<<(unsigned)((int64_t)a.units * a.heads), kPfThreads, PfSmem::kBytes, st>>>(mq, mkv, mkr, a);
+  latent_prefill_kernel<T><<<(unsigned)((int64_t)a.units * a.heads), kPfThreads, PfSmem::kBytes, st>>>(mq, mkv, mkr, mv,
+                                                                                                        a);
   return cudaGetLastError();
 }
 
