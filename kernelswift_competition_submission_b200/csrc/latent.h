@@ -1,4 +1,4 @@
-// Layout of the paged latent cache and launch helpers of the latent-attention units.
+// Layout of the paged latent cache, shared by the latent-attention units.
 //
 // A cached token is 512 latent values and a rotary key of 64. A 16-bit page holds page_size
 // rows of 576 elements. An e4m3 page of page_size * 644 bytes holds three parts, each
@@ -33,10 +33,5 @@ inline int64_t cache_page_bytes(int fmt, int page_size) {
 __device__ __forceinline__ float ue8m0_value(uint32_t code) {
   return code == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(code << 23);
 }
-
-cudaError_t launch_latent_decode16(int dtype, const void* q, int num_seqs, int q_len, int heads, const void* cache,
-                                   int64_t num_pages, int page_size, const int32_t* table, int64_t ld_table,
-                                   int table_width, const int32_t* lens, float scale, void* out, float* lse,
-                                   void* workspace, int* status, cudaStream_t st);
 
 }  // namespace moe

@@ -11,6 +11,8 @@
 //   warps 0-3  softmax: lane = row, warps 0-1 keys 0-63, warps 2-3 keys 64-127 of the tile; running
 //              maximum and sum, P into shared memory, O rescaled when the maximum has moved by 2^8
 //   warp 4     TMA producer: 16 KB slots ([64 keys][128 values]) in a ring of 8, in MMA order
+//   warps 6-13 (e4m3 pages) fill the slots instead of the TMA: codes from global memory into registers
+//              a whole tile ahead, widened to bf16 (exact: the scales are powers of two), stored swizzled
 //   warp 5     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
 //              beside PV of j - 1 and QK of j + 1
 //
@@ -37,7 +39,9 @@ constexpr int kDcRows = 64;           // rows per CTA
 constexpr int kDcSlots = 8;
 constexpr int kDcSlotBytes = 16384;   // [64 keys][128 values]
 constexpr int kDcMaxPairs = 80;
-constexpr int kDcThreads = 192;
+constexpr int kDcThreads = 192;       // 16-bit pages
+constexpr int kDcConv = 8;            // e4m3 pages: warps that widen the codes
+constexpr int kDcThreads8 = kDcThreads + 32 * kDcConv;
 constexpr float kDcRescaleLog2 = 8.0f;
 
 struct DcSmem {
@@ -142,7 +146,7 @@ __device__ __forceinline__ int row_seen(const DcArgs& a, int len, int r) {
 
 // One row by a warp, key by key over [kb, ke): maximum and sum in natural units, output unnormalised;
 // lane l holds the elements 2 l, 2 l + 1 of every 64.
-template <typename T>
+template <typename T, bool E4M3>
 __device__ __noinline__ void decode_row(const DcArgs& a, int b, int r, int kb, int ke, float& m, float& l,
                                         float (&acc)[16]) {
   const int lane = threadIdx.x & 31;
@@ -162,14 +166,33 @@ __device__ __noinline__ void decode_row(const DcArgs& a, int b, int r, int kb, i
   for (int j = kb; j < ke; ++j) {
     const int64_t page = __ldg(a.table + b * a.ld_table + (j >> a.page_shift));
     if (page < 0 || page >= a.num_pages) continue;
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(
-        a.cache + (page * a.page_size + (j & (a.page_size - 1))) * (int64_t)(2 * kRowDim));
+    const int off = j & (a.page_size - 1);
     float k[18], s = 0.f;
+    if constexpr (E4M3) {
+      const uint8_t* base = a.cache + page * ((int64_t)a.page_size * kRow8Bytes);
 #pragma unroll
-    for (int i = 0; i < 9; ++i) {
-      const float2 f = ElemTraits<T>::unpack2(__ldg(src + 32 * i + lane));
-      k[2 * i] = f.x;
-      k[2 * i + 1] = f.y;
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t c = __ldg(reinterpret_cast<const uint16_t*>(base + (int64_t)off * kLatDim + 64 * i) + lane);
+        const float sc =
+            ue8m0_value(__ldg(base + (int64_t)a.page_size * (kLatDim + 2 * kRopeDim) + off * 4 + (i >> 1)));
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        k[2 * i] = f.x * sc;
+        k[2 * i + 1] = f.y * sc;
+      }
+      const float2 f = ElemTraits<T>::unpack2(
+          __ldg(reinterpret_cast<const uint32_t*>(base + (int64_t)a.page_size * kLatDim + off * (2 * kRopeDim)) + lane));
+      k[16] = f.x;
+      k[17] = f.y;
+    } else {
+      const uint32_t* src =
+          reinterpret_cast<const uint32_t*>(a.cache + (page * a.page_size + off) * (int64_t)(2 * kRowDim));
+#pragma unroll
+      for (int i = 0; i < 9; ++i) {
+        const float2 f = ElemTraits<T>::unpack2(__ldg(src + 32 * i + lane));
+        k[2 * i] = f.x;
+        k[2 * i + 1] = f.y;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 18; ++i) s = fmaf(qv[i], k[i], s);
@@ -186,8 +209,67 @@ __device__ __noinline__ void decode_row(const DcArgs& a, int b, int r, int kb, i
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDcThreads, 1)
+// ---------------------------------------------------------------- e4m3 pages into 16-bit slots
+// The slots of one tile in MMA order: K0 K1 V0 K2 V1 ... over the run's segments.
+struct DcGroup {
+  int b, j, len, v;  // request, key tile, positions held; v: V (four slots), else K (five)
+};
+struct DcGroups {
+  DcIter it;
+  DcSeg sg;
+  int i, nt, next_k, next_v, seg;
+  __device__ __forceinline__ bool next(const DcArgs& a, DcGroup& g) {
+    if (next_v >= nt) {
+      if (!it.next(a, sg)) return false;
+      nt = sg.k1 - sg.k0;
+      next_k = next_v = 0;
+      ++seg;
+    }
+    g.b = sg.b;
+    g.len = sg.len;
+    g.v = next_k >= nt || next_k >= next_v + 2;
+    g.j = sg.k0 + (g.v ? next_v++ : next_k++);
+    return true;
+  }
+};
+// What a thread holds of one slot: 16 codes of two keys (or 16 bytes of their rotary values) and the scale bytes.
+struct DcRaw {
+  uint4 w[2];
+  uint32_t e[2];
+};
+
+// 16 codes times 2^(e - 127) as bf16.
+__device__ __forceinline__ void widen16(const uint4& q, uint32_t e, uint32_t (&o)[8]) {
+  const uint32_t c[4] = {q.x, q.y, q.z, q.w};
+  const uint32_t f = min(e + 120u, 254u) * 0x00800080u;  // bf16 2^(e - 7) in both halves, at most 2^127
+  uint32_t nan = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    nan |= (c[i] & 0x7F7F7F7Fu) + 0x01010101u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = __byte_perm(c[i], 0u, h ? 0x3424 : 0x1404);  // codes in the high bytes
+      const uint32_t b = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);  // the value times 2^-120
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(o[2 * i + h]) : "r"(b), "r"(f));
+    }
+  }
+  if (e > 134u) {
+    const uint32_t f2 = (e - 7u) * 0x00800080u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f2));
+  }
+  if (nan & 0x80808080u) {  // e4m3 NaN came out as 480
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = c[i >> 1] >> (16 * (i & 1));
+      if ((w & 0x7Fu) == 0x7Fu) o[i] = (o[i] & 0xFFFF0000u) | 0x7FC0u;
+      if ((w & 0x7F00u) == 0x7F00u) o[i] = (o[i] & 0xFFFFu) | 0x7FC00000u;
+    }
+  }
+}
+
+template <typename T, bool E4M3>
+__global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
 latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
                      const __grid_constant__ DcArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -248,7 +330,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 2 * kDcConv : 1); mbar_init(&empty[s], 1); }
     mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(&s_full[0], 1);
@@ -404,6 +486,10 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
       }
       __syncwarp();
+      if constexpr (E4M3) {
+        ++seg;
+        continue;
+      }
       int pg0 = pages_of(sg, sg.k0), pg1 = pages_of(sg, sg.k0 + 1), pg2 = pages_of(sg, sg.k0 + 2);
       ok = load_k(pg0, sg.k0);
       if (ok && sg.k0 + 1 < sg.k1) ok = load_k(pg1, sg.k0 + 1);
@@ -473,7 +559,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (nt <= 2) free_q();
         for (int j = 0; j < nt && ok; ++j) {
           if (j == 0 && seg > 0) ok = mbar_wait_warp(o_free, (seg - 1) & 1, a.status, s_abort) && ok;
-          if ((sg.k0 + j + 1) * kDcTile > sure) {
+          if (!E4M3 && (sg.k0 + j + 1) * kDcTile > sure) {
             ok = mbar_wait_warp(v_fixed, n_fixed & 1, a.status, s_abort) && ok;
             ++n_fixed;
           }
@@ -504,6 +590,126 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       if (one) umma_commit_pair(mma_done);  // every MMA issued here is done before TMEM is freed
       __syncwarp();
       mbar_wait_warp(mma_done, 0, nullptr, nullptr);
+    }
+  } else if (E4M3 && warp >= 6) {
+    // ------------------------------------------------ slots from e4m3 pages
+    const int t = threadIdx.x - kDcThreads;     // 0 .. 255
+    const int key_lo = t >> 3, part = t & 7;    // keys key_lo and key_lo + 32 of 64, 16 of 128 values
+    const uint32_t full0 = mapa_shared(full, 0);
+    DcGroups gen{it, {}, 0, 0, 0, 0, 0};
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto pages_of = [&](const DcGroup& g, int (&pg)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t key = (int64_t)g.j * kDcTile + i * 32 + key_lo;
+        const int64_t pi = key >> a.page_shift;
+        const int p = key < g.len ? __ldg(a.table + g.b * a.ld_table + pi) : -1;
+        pg[i] = p < a.num_pages ? p : -1;  // below zero: zeros in the slot
+      }
+    };
+    auto fetch = [&](const DcGroup& g, const int (&pg)[4], DcRaw (&raw)[5]) {
+#pragma unroll
+      for (int c = 0; c < 5; ++c) {
+        if (c < 4 || !g.v) {
+          const int half = g.v ? (c & 1) : (int)rank, blk = g.v ? 2 * (c >> 1) + (int)rank : c;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int p = half ? pg[2 + u] : pg[u];
+            raw[c].w[u] = make_uint4(0u, 0u, 0u, 0u);
+            raw[c].e[u] = 127u;
+            if (p >= 0) {
+              const int off = (g.j * kDcTile + half * 64 + u * 32 + key_lo) & (a.page_size - 1);
+              const uint8_t* base = a.cache + (int64_t)p * ((int64_t)a.page_size * kRow8Bytes);
+              if (c < 4) {
+                raw[c].w[u] = __ldg(reinterpret_cast<const uint4*>(base + off * kLatDim + blk * kLatBlk) + part);
+                raw[c].e[u] = __ldg(base + a.page_size * (kLatDim + 2 * kRopeDim) + off * 4 + blk);
+              } else {
+                raw[c].w[u] = __ldg(reinterpret_cast<const uint4*>(base + a.page_size * kLatDim + off * (2 * kRopeDim)) + part);
+              }
+            }
+          }
+        }
+      }
+    };
+    auto fill = [&](const DcGroup& g, const DcRaw (&raw)[5], int seg) {
+      // values that some query may not see must not be NaN under its P = 0
+      const int sure = max(0, g.len - a.n_q + 1);
+      const bool watch = g.v && (g.j + 1) * kDcTile > sure;
+#pragma unroll
+      for (int c = 0; c < 5; ++c) {
+        if (c < 4 || !g.v) {
+          ok = mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort) && ok;
+          uint8_t* base = ring + slot * kDcSlotBytes;
+          bool bad = false;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int key = u * 32 + key_lo;
+            if (c < 4) {
+              uint32_t o[8];
+              widen16(raw[c].w[u], raw[c].e[u], o);
+              // 32 bytes of chunk part / 4; the two halves in an order that keeps eight lanes on eight banks
+              uint8_t* row = base + (part >> 2) * 8192 + key * 128;
+              const int un = (part & 3) * 2, sw = part >> 2;
+              const uint4 v0 = make_uint4(o[0], o[1], o[2], o[3]), v1 = make_uint4(o[4], o[5], o[6], o[7]);
+              *reinterpret_cast<uint4*>(row + (((un + sw) ^ (key & 7)) << 4)) = sw ? v1 : v0;
+              *reinterpret_cast<uint4*>(row + (((un + 1 - sw) ^ (key & 7)) << 4)) = sw ? v0 : v1;
+              if (watch && g.j * kDcTile + (c & 1) * 64 + key >= sure) {
+                const uint32_t w[4] = {raw[c].w[u].x, raw[c].w[u].y, raw[c].w[u].z, raw[c].w[u].w};
+                uint32_t nan = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) nan |= (w[i] & 0x7F7F7F7Fu) + 0x01010101u;
+                bad |= (nan & 0x80808080u) != 0u;
+              }
+            } else {
+              *reinterpret_cast<uint4*>(base + key * 128 + ((part ^ (key & 7)) << 4)) = raw[c].w[u];
+            }
+          }
+          if (watch && __any_sync(0xffffffffu, bad) && lane < 2) {
+            const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
+          if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+        }
+      }
+    };
+    // pages two groups ahead, codes one group ahead of the stores
+    DcGroup g0, g1, g2;
+    int pg1[4], pg2[4];
+    DcRaw cur[5], nxt[5];
+    gen.seg = -1;
+    bool h0 = gen.next(a, g0);
+    int s0 = gen.seg, s1 = 0, s2 = 0;
+    bool h1 = false, h2 = false;
+    if (h0) {
+      pages_of(g0, pg1);
+      fetch(g0, pg1, cur);
+      h1 = gen.next(a, g1);
+      s1 = gen.seg;
+      if (h1) pages_of(g1, pg1);
+    }
+    while (h0 && ok) {
+      if (h1) {
+        fetch(g1, pg1, nxt);
+        h2 = gen.next(a, g2);
+        s2 = gen.seg;
+        if (h2) pages_of(g2, pg2);
+      }
+      fill(g0, cur, s0);
+      g0 = g1;
+      g1 = g2;
+      h0 = h1;
+      h1 = h1 && h2;
+      s0 = s1;
+      s1 = s2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pg1[i] = pg2[i];
+#pragma unroll
+      for (int c = 0; c < 5; ++c) cur[c] = nxt[c];
     }
   } else {
     // ------------------------------------------------ softmax
@@ -644,7 +850,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const int rw = sg.rt * kDcTile + (int)rank * kDcRows + rr;
           if (rw >= a.rows) break;
           float m, ls, acc[16];
-          decode_row<T>(a, sg.b, rw, sg.k0 * kDcTile, min(row_seen(a, sg.len, rw), sg.k1 * kDcTile), m, ls, acc);
+          decode_row<T, E4M3>(a, sg.b, rw, sg.k0 * kDcTile, min(row_seen(a, sg.len, rw), sg.k1 * kDcTile), m, ls, acc);
           const bool some = ls > 0.f || ls != ls;
           if (whole) {
             const int64_t o = (int64_t)sg.b * a.rows + rw;
@@ -804,7 +1010,7 @@ cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
   return cudaSuccess;
 }
 
-template <typename T>
+template <typename T, bool E4M3>
 cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   CUtensorMap mq, mc;
   const uint64_t row = 2 * kRowDim;
@@ -813,10 +1019,10 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
   const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
   const uint32_t box_rows = (uint32_t)std::min(a.page_size, 64);
-  if (!make_chunks_map(&mq, dtype, a.q, dq, sq, kDcRows, kRowDim / 64) ||
-      !make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1))
-    return cudaErrorInvalidValue;
-  auto kern = latent_decode_kernel<T>;
+  if (!make_chunks_map(&mq, dtype, a.q, dq, sq, kDcRows, kRowDim / 64)) return cudaErrorInvalidValue;
+  if (E4M3) mc = mq;  // the codes are not read by TMA
+  else if (!make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1)) return cudaErrorInvalidValue;
+  auto kern = latent_decode_kernel<T, E4M3>;
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(kern), DcSmem::kBytes);
   if (err != cudaSuccess) return err;
   cudaLaunchAttribute attr[1];
@@ -825,7 +1031,7 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kDcThreads, 1, 1);
+  cfg.blockDim = dim3(E4M3 ? kDcThreads8 : kDcThreads, 1, 1);
   cfg.dynamicSmemBytes = DcSmem::kBytes;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -837,23 +1043,48 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-}  // namespace
+inline bool al16d(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-cudaError_t launch_latent_decode16(int dtype, const void* q, int num_seqs, int q_len, int heads, const void* cache,
-                                   int64_t num_pages, int page_size, const int32_t* table, int64_t ld_table,
-                                   int table_width, const int32_t* lens, float scale, void* out, float* lse,
-                                   void* workspace, int* status, cudaStream_t st) {
+}  // namespace
+}  // namespace moe
+
+extern "C" size_t moe_latent_decode_workspace_bytes(int64_t num_seqs, int q_len, int heads) {
+  if (num_seqs < 0 || q_len <= 0 || heads <= 0) return 0;
+  const size_t rows = (size_t)std::min<int64_t>((int64_t)q_len * heads, moe::kDcTile);
+  return 2 * (size_t)moe::kDcMaxPairs * rows * (moe::kLatDim * 4 + 8);
+}
+
+extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int q_len, int heads, int cache_fmt,
+                                 const void* cache, int64_t num_pages, int page_size, const int32_t* block_table,
+                                 int64_t ld_table, int table_width, const int32_t* cache_lens, float scale, void* out,
+                                 float* lse, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  using namespace moe;
+  if (!cache_fmt_ok(cache_fmt) || (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_FP16)) return MOE_ERR_UNSUPPORTED;
+  if (cache_fmt == MOE_CACHE_E4M3 ? dtype != MOE_DTYPE_BF16 : dtype != cache_fmt) return MOE_ERR_UNSUPPORTED;
+  if (num_seqs < 0 || q_len <= 0 || heads <= 0 || num_pages < 0 || table_width < 0 || ld_table < 0)
+    return MOE_ERR_INVALID_ARG;
+  if (!page_size_ok(page_size) || num_pages > INT32_MAX || (int64_t)q_len * heads > 65536 || num_seqs > 65535 ||
+      (int64_t)table_width * page_size > INT32_MAX - kDcTile)
+    return MOE_ERR_BAD_SHAPE;
+  if (num_seqs == 0) return MOE_OK;
+  if (num_pages == 0 || !q || !cache || !cache_lens || !out || (table_width > 0 && !block_table))
+    return MOE_ERR_INVALID_ARG;
+  if (!al16d(q) || !al16d(cache) || !al16d(out)) return MOE_ERR_INVALID_ARG;
+  if (workspace_bytes < moe_latent_decode_workspace_bytes(num_seqs, q_len, heads) || !workspace || !al16d(workspace))
+    return MOE_ERR_WORKSPACE;
+  const int rc = moe_check_device();
+  if (rc != MOE_OK) return rc;
   DcArgs a{};
   a.q = q;
   a.cache = static_cast<const uint8_t*>(cache);
-  a.table = table;
+  a.table = block_table;
   a.ld_table = ld_table;
-  a.lens = lens;
+  a.lens = cache_lens;
   a.num_pages = num_pages;
   a.table_width = table_width;
   a.page_size = page_size;
   a.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
-  a.num_seqs = num_seqs;
+  a.num_seqs = (int)num_seqs;
   a.n_q = q_len;
   a.heads = heads;
   a.rows = q_len * heads;
@@ -868,13 +1099,9 @@ cudaError_t launch_latent_decode16(int dtype, const void* q, int num_seqs, int q
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + 2 * (size_t)kDcMaxPairs * a.part_rows * kLatDim);
   a.status = status;
-  return dtype == MOE_DTYPE_BF16 ? launch_decode<__nv_bfloat16>(dtype, a, st) : launch_decode<__half>(dtype, a, st);
-}
-
-}  // namespace moe
-
-extern "C" size_t moe_latent_decode_workspace_bytes(int64_t num_seqs, int q_len, int heads) {
-  if (num_seqs < 0 || q_len <= 0 || heads <= 0) return 0;
-  const size_t rows = (size_t)std::min<int64_t>((int64_t)q_len * heads, moe::kDcTile);
-  return 2 * (size_t)moe::kDcMaxPairs * rows * (moe::kLatDim * 4 + 8);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = cache_fmt == MOE_CACHE_E4M3   ? launch_decode<__nv_bfloat16, true>(dtype, a, st)
+                          : dtype == MOE_DTYPE_BF16 ? launch_decode<__nv_bfloat16, false>(dtype, a, st)
+                                                    : launch_decode<__half, false>(dtype, a, st);
+  return err == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
