@@ -136,6 +136,13 @@ __device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* ba
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+// Untiled bulk copy: both addresses and the size are multiples of 16.
+__device__ __forceinline__ void bulk_load(const void* src, uint64_t* bar, void* dst, uint32_t bytes) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
 
 // ---------------------------------------------------------------- cp.async (16-byte, L2 only)
 // Copies 16 bytes global -> shared; src_bytes = 0 reads nothing and writes zeros.

@@ -11,8 +11,8 @@
 //   warps 0-3  softmax: lane = row, warps 0-1 keys 0-63, warps 2-3 keys 64-127 of the tile; running
 //              maximum and sum, P into shared memory, O rescaled when the maximum has moved by 2^8
 //   warp 4     TMA producer: 16 KB slots ([64 keys][128 values]) in a ring of 8, in MMA order
-//   warps 6-13 (e4m3 pages) fill the slots instead of the TMA: codes from global memory into registers
-//              a whole tile ahead, widened to bf16 (exact: the scales are powers of two), stored swizzled
+//   warps 6-13 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
+//              (exact: the scales are powers of two), two warps a slot
 //   warp 5     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
 //              beside PV of j - 1 and QK of j + 1
 //
@@ -48,9 +48,10 @@ struct DcSmem {
   static constexpr int kRing = 9 * 8192;                      // after Q: nine [64 rows][64] chunks
   static constexpr int kP = kRing + kDcSlots * kDcSlotBytes;  // two [64 rows][64 keys] chunks
   static constexpr int kX = kP + 16384;                       // row maxima / sums of both key halves, two tiles
-  static constexpr int kBars = kX + 2 * 128 * 4;
-  // full[8], empty[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix, v_fixed
-  static constexpr int kNumBars = 2 * kDcSlots + 10;
+  static constexpr int kScales = kX + 2 * 128 * 4;            // e4m3: four scale bytes of a slot's 64 keys
+  static constexpr int kBars = kScales + kDcSlots * 256;
+  // full[8], empty[8], raw[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix, v_fixed
+  static constexpr int kNumBars = 3 * kDcSlots + 10;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kBytes = kMisc + 64 + 1024;
 };
@@ -232,14 +233,8 @@ struct DcGroups {
     return true;
   }
 };
-// What a thread holds of one slot: 16 codes of two keys (or 16 bytes of their rotary values) and the scale bytes.
-struct DcRaw {
-  uint4 w[2];
-  uint32_t e[2];
-};
-
-// 16 codes times 2^(e - 127) as bf16.
-__device__ __forceinline__ void widen16(const uint4& q, uint32_t e, uint32_t (&o)[8]) {
+// 16 codes times 2^(e - 127) as bf16; true when one is NaN.
+__device__ __forceinline__ bool widen16(const uint4& q, uint32_t e, uint32_t (&o)[8]) {
   const uint32_t c[4] = {q.x, q.y, q.z, q.w};
   const uint32_t f = min(e + 120u, 254u) * 0x00800080u;  // bf16 2^(e - 7) in both halves, at most 2^127
   uint32_t nan = 0;
@@ -265,13 +260,15 @@ __device__ __forceinline__ void widen16(const uint4& q, uint32_t e, uint32_t (&o
       if ((w & 0x7Fu) == 0x7Fu) o[i] = (o[i] & 0xFFFF0000u) | 0x7FC0u;
       if ((w & 0x7F00u) == 0x7F00u) o[i] = (o[i] & 0xFFFFu) | 0x7FC00000u;
     }
+    return true;
   }
+  return false;
 }
 
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
 latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
-                     const __grid_constant__ DcArgs a) {
+                     const __grid_constant__ CUtensorMap map_r, const __grid_constant__ DcArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + DcSmem::kRing;
@@ -280,7 +277,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + DcSmem::kBars);
   uint64_t* full = bars;                 // first CTA's: both CTAs' copies of a slot
   uint64_t* empty = full + kDcSlots;     // each CTA's
-  uint64_t* q_full = empty + kDcSlots;   // first CTA's
+  uint64_t* raw = empty + kDcSlots;      // each CTA's, e4m3: codes and scales of a slot
+  uint64_t* q_full = raw + kDcSlots;     // first CTA's
   uint64_t* q_free = q_full + 1;
   uint64_t* s_full = q_free + 1;         // [2]
   uint64_t* p_full = s_full + 2;         // first CTA's: eight softmax warps
@@ -330,7 +328,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 2 * kDcConv : 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 4 : 1); mbar_init(&empty[s], 1); mbar_init(&raw[s], 1); }
     mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(&s_full[0], 1);
@@ -398,6 +396,34 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       if (rank == 0 && one) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
       __syncwarp();
     };
+    // e4m3: 64 keys of tile j into the slot as they are, codes of value block blk with their scale bytes, or
+    // (blk 4) the rotary keys, which need no widening. Bytes are counted on this CTA's raw[slot].
+    auto copy_raw = [&](int pages, int half, int j, int blk) {
+      uint8_t* dst = ring + slot * kDcSlotBytes;
+      uint8_t* sdst = smem + DcSmem::kScales + slot * 256;
+      const int row = br == 64 ? (j * kDcTile + half * 64) & (a.page_size - 1) : 0;
+      uint32_t bytes = 8192;
+      if (blk < 4)
+        for (int i = 0; i < ppk; ++i) {
+          const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
+          if (page >= 0 && page < a.num_pages) bytes += br * 4;  // a page outside the cache has no scales
+        }
+      if (one) mbar_arrive_expect_tx(&raw[slot], bytes);
+      for (int i = 0; i < ppk; ++i) {
+        const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
+        if (one) {
+          if (blk < 4) {
+            tma_load_3d(&map_c, &raw[slot], dst + i * br * 128, blk * 128, row, page);
+            if (page >= 0 && page < a.num_pages)
+              bulk_load(a.cache + (int64_t)page * (a.page_size * kRow8Bytes) + a.page_size * (kLatDim + 2 * kRopeDim) + row * 4,
+                        &raw[slot], sdst + i * br * 4, br * 4);
+          } else {
+            tma_load_3d(&map_r, &raw[slot], dst + i * br * 128, 0, row, page);
+          }
+        }
+        __syncwarp();
+      }
+    };
     auto step = [&]() {
       issued |= 1u << slot;
       issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
@@ -406,8 +432,12 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     auto load_k = [&](int pages, int j) {
       for (int c = 0; c < 5; ++c) {
         if (!wait_empty()) return false;
-        announce(kDcSlotBytes);
-        copy(pages, (int)rank, j, c * 2, false);
+        if constexpr (E4M3) {
+          copy_raw(pages, (int)rank, j, c);
+        } else {
+          announce(kDcSlotBytes);
+          copy(pages, (int)rank, j, c * 2, false);
+        }
         step();
       }
       return true;
@@ -415,11 +445,15 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     auto load_v = [&](const DcSeg& s, int pages, int j) {
       // slot order: value block 0 keys 0-63, 64-127, value block 1 keys 0-63, 64-127
       const int sure = max(0, s.len - a.n_q + 1);  // keys that every row sees
-      if ((j + 1) * kDcTile <= sure) {
+      if (E4M3 || (j + 1) * kDcTile <= sure) {
         for (int c = 0; c < 4; ++c) {
           if (!wait_empty()) return false;
-          announce(kDcSlotBytes);
-          copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, false);
+          if constexpr (E4M3) {
+            copy_raw(pages, c & 1, j, (c >> 1) * 2 + (int)rank);
+          } else {
+            announce(kDcSlotBytes);
+            copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, false);
+          }
           step();
         }
         return true;
@@ -486,10 +520,6 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
       }
       __syncwarp();
-      if constexpr (E4M3) {
-        ++seg;
-        continue;
-      }
       int pg0 = pages_of(sg, sg.k0), pg1 = pages_of(sg, sg.k0 + 1), pg2 = pages_of(sg, sg.k0 + 2);
       ok = load_k(pg0, sg.k0);
       if (ok && sg.k0 + 1 < sg.k1) ok = load_k(pg1, sg.k0 + 1);
@@ -503,9 +533,9 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       ++seg;
     }
-    if (!ok && rank == 0) {  // wait (bounded) for copies in flight before the pair may leave
+    if (!ok && (E4M3 || rank == 0)) {  // wait (bounded) for copies in flight before the pair may leave
       for (int s = 0; s < kDcSlots; ++s)
-        if ((issued >> s) & 1u) mbar_wait_warp(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+        if ((issued >> s) & 1u) mbar_wait_warp(E4M3 ? &raw[s] : &full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
     }
   } else if (warp == 5) {
     if (rank == 0) {
@@ -592,124 +622,65 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       mbar_wait_warp(mma_done, 0, nullptr, nullptr);
     }
   } else if (E4M3 && warp >= 6) {
-    // ------------------------------------------------ slots from e4m3 pages
-    const int t = threadIdx.x - kDcThreads;     // 0 .. 255
-    const int key_lo = t >> 3, part = t & 7;    // keys key_lo and key_lo + 32 of 64, 16 of 128 values
+    // ------------------------------------------------ e4m3 codes to bf16, in place
+    // Two warps per slot, four slots at a time, so that one team's waits lie beside the others' work. The
+    // codes come into the first half of the slot; a team takes them into registers, then writes all of it.
+    const int t = threadIdx.x & 63;             // of the team's 64 threads
+    const int team = (warp - 6) >> 1;           // the run's slots team, team + 4, ...
+    const int key_lo = t >> 3, part = t & 7;    // keys key_lo + 8 u, 16 of 128 values
     const uint32_t full0 = mapa_shared(full, 0);
-    DcGroups gen{it, {}, 0, 0, 0, 0, 0};
-    int slot = 0;
+    DcGroups gen{it, {}, 0, 0, 0, 0, -1};
+    DcGroup grp;
+    int c = team, slot = team;                  // slot of the tile's K or V, and of the ring
     uint32_t phase = 0;
     bool ok = true;
-    auto pages_of = [&](const DcGroup& g, int (&pg)[4]) {
+    bool more = gen.next(a, grp);
+    while (more && ok) {
+      const int half = grp.v ? (c & 1) : (int)rank, blk = grp.v ? 2 * (c >> 1) + (int)rank : c;
+      const int first = grp.j * kDcTile + half * 64;
+      uint8_t* base = ring + slot * kDcSlotBytes;
+      ok = mbar_wait_warp(&raw[slot], phase, a.status, s_abort);
+      if (blk < 4) {
+        const uint8_t* sc = smem + DcSmem::kScales + slot * 256 + blk;
+        uint4 w[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t key = (int64_t)g.j * kDcTile + i * 32 + key_lo;
-        const int64_t pi = key >> a.page_shift;
-        const int p = key < g.len ? __ldg(a.table + g.b * a.ld_table + pi) : -1;
-        pg[i] = p < a.num_pages ? p : -1;  // below zero: zeros in the slot
-      }
-    };
-    auto fetch = [&](const DcGroup& g, const int (&pg)[4], DcRaw (&raw)[5]) {
+        for (int u = 0; u < 8; ++u) w[u] = *reinterpret_cast<const uint4*>(base + (8 * u + key_lo) * 128 + part * 16);
+        named_bar_sync(2 + team, 64);  // all codes are in registers
+        // the next group's segment may be read meanwhile
+        const int sure = max(0, grp.len - a.n_q + 1);
+        bool bad = false;
+        const int sw = part >> 2;
+        uint8_t* row = base + sw * 8192 + key_lo * 128;
+        // this thread's 32 bytes of chunk part / 4: the two halves in an order that keeps eight lanes on eight banks
+        const uint32_t o0 = (uint32_t)((((part & 3) * 2 + sw) ^ key_lo) << 4), o1 = (uint32_t)((((part & 3) * 2 + 1 - sw) ^ key_lo) << 4);
 #pragma unroll
-      for (int c = 0; c < 5; ++c) {
-        if (c < 4 || !g.v) {
-          const int half = g.v ? (c & 1) : (int)rank, blk = g.v ? 2 * (c >> 1) + (int)rank : c;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int p = half ? pg[2 + u] : pg[u];
-            raw[c].w[u] = make_uint4(0u, 0u, 0u, 0u);
-            raw[c].e[u] = 127u;
-            if (p >= 0) {
-              const int off = (g.j * kDcTile + half * 64 + u * 32 + key_lo) & (a.page_size - 1);
-              const uint8_t* base = a.cache + (int64_t)p * ((int64_t)a.page_size * kRow8Bytes);
-              if (c < 4) {
-                raw[c].w[u] = __ldg(reinterpret_cast<const uint4*>(base + off * kLatDim + blk * kLatBlk) + part);
-                raw[c].e[u] = __ldg(base + a.page_size * (kLatDim + 2 * kRopeDim) + off * 4 + blk);
-              } else {
-                raw[c].w[u] = __ldg(reinterpret_cast<const uint4*>(base + a.page_size * kLatDim + off * (2 * kRopeDim)) + part);
-              }
-            }
-          }
+        for (int u = 0; u < 8; ++u) {
+          const int key = first + 8 * u + key_lo;
+          uint32_t o[8];
+          if (key >= grp.len) w[u] = make_uint4(0u, 0u, 0u, 0u);
+          const bool nan = widen16(w[u], sc[(8 * u + key_lo) * 4], o);
+          bad |= nan && key >= sure;
+          const uint4 v0 = make_uint4(o[0], o[1], o[2], o[3]), v1 = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(row + u * 1024 + o0) = sw ? v1 : v0;
+          *reinterpret_cast<uint4*>(row + u * 1024 + o1) = sw ? v0 : v1;
         }
-      }
-    };
-    auto fill = [&](const DcGroup& g, const DcRaw (&raw)[5], int seg) {
-      // values that some query may not see must not be NaN under its P = 0
-      const int sure = max(0, g.len - a.n_q + 1);
-      const bool watch = g.v && (g.j + 1) * kDcTile > sure;
-#pragma unroll
-      for (int c = 0; c < 5; ++c) {
-        if (c < 4 || !g.v) {
-          ok = mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort) && ok;
-          uint8_t* base = ring + slot * kDcSlotBytes;
-          bool bad = false;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int key = u * 32 + key_lo;
-            if (c < 4) {
-              uint32_t o[8];
-              widen16(raw[c].w[u], raw[c].e[u], o);
-              // 32 bytes of chunk part / 4; the two halves in an order that keeps eight lanes on eight banks
-              uint8_t* row = base + (part >> 2) * 8192 + key * 128;
-              const int un = (part & 3) * 2, sw = part >> 2;
-              const uint4 v0 = make_uint4(o[0], o[1], o[2], o[3]), v1 = make_uint4(o[4], o[5], o[6], o[7]);
-              *reinterpret_cast<uint4*>(row + (((un + sw) ^ (key & 7)) << 4)) = sw ? v1 : v0;
-              *reinterpret_cast<uint4*>(row + (((un + 1 - sw) ^ (key & 7)) << 4)) = sw ? v0 : v1;
-              if (watch && g.j * kDcTile + (c & 1) * 64 + key >= sure) {
-                const uint32_t w[4] = {raw[c].w[u].x, raw[c].w[u].y, raw[c].w[u].z, raw[c].w[u].w};
-                uint32_t nan = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) nan |= (w[i] & 0x7F7F7F7Fu) + 0x01010101u;
-                bad |= (nan & 0x80808080u) != 0u;
-              }
-            } else {
-              *reinterpret_cast<uint4*>(base + key * 128 + ((part ^ (key & 7)) << 4)) = raw[c].w[u];
-            }
-          }
-          if (watch && __any_sync(0xffffffffu, bad) && lane < 2) {
-            const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
-          if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+        // values that some query may not see must not be NaN under its P = 0
+        if (grp.v && __any_sync(0xffffffffu, bad) && lane < 2) {
+          const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (gen.seg & 1), (uint32_t)lane);
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(gen.seg + 1) : "memory");
         }
+        fence_proxy_async_smem();
       }
-    };
-    // pages two groups ahead, codes one group ahead of the stores
-    DcGroup g0, g1, g2;
-    int pg1[4], pg2[4];
-    DcRaw cur[5], nxt[5];
-    gen.seg = -1;
-    bool h0 = gen.next(a, g0);
-    int s0 = gen.seg, s1 = 0, s2 = 0;
-    bool h1 = false, h2 = false;
-    if (h0) {
-      pages_of(g0, pg1);
-      fetch(g0, pg1, cur);
-      h1 = gen.next(a, g1);
-      s1 = gen.seg;
-      if (h1) pages_of(g1, pg1);
-    }
-    while (h0 && ok) {
-      if (h1) {
-        fetch(g1, pg1, nxt);
-        h2 = gen.next(a, g2);
-        s2 = gen.seg;
-        if (h2) pages_of(g2, pg2);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
+      slot ^= 4;  // the team's other slot of the ring
+      if (slot < 4) phase ^= 1;
+      c += 4;
+      const int n = grp.v ? 4 : 5;
+      if (c >= n) {
+        c -= n;
+        more = gen.next(a, grp);
       }
-      fill(g0, cur, s0);
-      g0 = g1;
-      g1 = g2;
-      h0 = h1;
-      h1 = h1 && h2;
-      s0 = s1;
-      s1 = s2;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pg1[i] = pg2[i];
-#pragma unroll
-      for (int c = 0; c < 5; ++c) cur[c] = nxt[c];
     }
   } else {
     // ------------------------------------------------ softmax
@@ -1012,16 +983,25 @@ cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
 
 template <typename T, bool E4M3>
 cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
-  CUtensorMap mq, mc;
+  CUtensorMap mq, mc, mr;
   const uint64_t row = 2 * kRowDim;
   const uint64_t dq[4] = {64, (uint64_t)a.rows, kRowDim / 64, (uint64_t)a.num_seqs};
   const uint64_t sq[3] = {row, 128, row * (uint64_t)a.rows};
-  const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
-  const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
   const uint32_t box_rows = (uint32_t)std::min(a.page_size, 64);
-  if (!make_chunks_map(&mq, dtype, a.q, dq, sq, kDcRows, kRowDim / 64)) return cudaErrorInvalidValue;
-  if (E4M3) mc = mq;  // the codes are not read by TMA
-  else if (!make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1)) return cudaErrorInvalidValue;
+  const uint64_t page8 = (uint64_t)a.page_size * kRow8Bytes;
+  bool maps = make_chunks_map(&mq, dtype, a.q, dq, sq, kDcRows, kRowDim / 64);
+  if (E4M3) {
+    const uint64_t dc[3] = {kLatDim, (uint64_t)a.page_size, (uint64_t)a.num_pages}, sc[2] = {kLatDim, page8};
+    const uint64_t dr[3] = {kRopeDim, (uint64_t)a.page_size, (uint64_t)a.num_pages}, sr[2] = {2 * kRopeDim, page8};
+    maps = maps && make_bytes_map(&mc, a.cache, dc, sc, box_rows) &&
+           make_kmajor_map(&mr, dtype, a.cache + (size_t)a.page_size * kLatDim, 3, dr, sr, box_rows);
+  } else {
+    const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
+    const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
+    maps = maps && make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1);
+    mr = mc;
+  }
+  if (!maps) return cudaErrorInvalidValue;
   auto kern = latent_decode_kernel<T, E4M3>;
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(kern), DcSmem::kBytes);
   if (err != cudaSuccess) return err;
@@ -1038,7 +1018,7 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   cfg.numAttrs = 1;
   if ((err = resident_pairs(kern, cfg, &a.pairs)) != cudaSuccess) return err;
   cfg.gridDim = dim3(2 * (unsigned)a.pairs, 1, 1);
-  if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, a)) != cudaSuccess) return err;
+  if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, mr, a)) != cudaSuccess) return err;
   latent_decode_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.num_seqs * a.rows, 4), 128, 0, st>>>(a);
   return cudaGetLastError();
 }
