@@ -233,36 +233,31 @@ struct DcGroups {
     return true;
   }
 };
-// 16 codes times 2^(e - 127) as bf16; true when one is NaN.
-__device__ __forceinline__ bool widen16(const uint4& q, uint32_t e, uint32_t (&o)[8]) {
-  const uint32_t c[4] = {q.x, q.y, q.z, q.w};
-  const uint32_t f = min(e + 120u, 254u) * 0x00800080u;  // bf16 2^(e - 7) in both halves, at most 2^127
-  uint32_t nan = 0;
+// 8 codes times 2^(e - 127) as bf16: f is bf16 2^min(e - 7, 127) in both halves, f2 what is left of it
+// (e above 134 only). The codes' exponent and fraction moved to the low end of bf16's are the value times
+// 2^-120, subnormals included, and the multiply rounds nothing. Bit 7 of a byte of `nan`: a NaN code, which
+// comes out as 480 here.
+__device__ __forceinline__ void widen8(uint2 q, uint32_t f, bool big, uint32_t f2, uint32_t& nan, uint32_t (&o)[4]) {
+  const uint32_t c[2] = {q.x, q.y};
+  nan |= ((c[0] & 0x7F7F7F7Fu) + 0x01010101u) | ((c[1] & 0x7F7F7F7Fu) + 0x01010101u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    nan |= (c[i] & 0x7F7F7F7Fu) + 0x01010101u;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t w = __byte_perm(c[i], 0u, h ? 0x3424 : 0x1404);  // codes in the high bytes
-      const uint32_t b = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);  // the value times 2^-120
-      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(o[2 * i + h]) : "r"(b), "r"(f));
-    }
+    const uint32_t w = __byte_perm(c[i >> 1], 0u, (i & 1) ? 0x3424 : 0x1404);  // two codes in the high bytes
+    const uint32_t b = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(o[i]) : "r"(b), "r"(f));
   }
-  if (e > 134u) {
-    const uint32_t f2 = (e - 7u) * 0x00800080u;
+  if (big) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f2));
+    for (int i = 0; i < 4; ++i) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(o[i]) : "r"(f2));
   }
-  if (nan & 0x80808080u) {  // e4m3 NaN came out as 480
+}
+__device__ __forceinline__ void nan8(uint2 q, uint32_t (&o)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w = c[i >> 1] >> (16 * (i & 1));
-      if ((w & 0x7Fu) == 0x7Fu) o[i] = (o[i] & 0xFFFF0000u) | 0x7FC0u;
-      if ((w & 0x7F00u) == 0x7F00u) o[i] = (o[i] & 0xFFFFu) | 0x7FC00000u;
-    }
-    return true;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = ((i >> 1) ? q.y : q.x) >> (16 * (i & 1));
+    if ((w & 0x7Fu) == 0x7Fu) o[i] = (o[i] & 0xFFFF0000u) | 0x7FC0u;
+    if ((w & 0x7F00u) == 0x7F00u) o[i] = (o[i] & 0xFFFFu) | 0x7FC00000u;
   }
-  return false;
 }
 
 template <typename T, bool E4M3>
@@ -399,7 +394,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     // e4m3: 64 keys of tile j into the slot as they are, codes of value block blk with their scale bytes, or
     // (blk 4) the rotary keys, which need no widening. Bytes are counted on this CTA's raw[slot].
     auto copy_raw = [&](int pages, int half, int j, int blk) {
-      uint8_t* dst = ring + slot * kDcSlotBytes;
+      uint8_t* dst = ring + slot * kDcSlotBytes + (blk < 4 ? 8192 : 0);
       uint8_t* sdst = smem + DcSmem::kScales + slot * 256;
       const int row = br == 64 ? (j * kDcTile + half * 64) & (a.page_size - 1) : 0;
       uint32_t bytes = 8192;
@@ -557,15 +552,17 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       };
       auto issue_qk = [&](int tile) {
         const uint32_t d = tmem + kTmemS + (tile & 1) * 64;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 5; ++c) {
           take();
           if (one) {
-            const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4);
+            const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4), da = dq0 + c * (16384 >> 4);
 #pragma unroll
-            for (int k = 0; k < (c < 4 ? 8 : 4); ++k) {
-              const uint32_t step = (k >> 2) * (8192 >> 4) + 2 * (k & 3);
-              umma_f16_pair(d, dq0 + c * (16384 >> 4) + step, db + step, kIdescQK, (c | k) != 0);
+            for (int k = 0; k < 4; ++k) umma_f16_pair(d, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
+            if (c < 4) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16_pair(d, da + (8192 >> 4) + 2 * k, db + (8192 >> 4) + 2 * k, kIdescQK, 1);
             }
             umma_commit_pair_multicast(&empty[slot], 0x3);
             if (c == 4) umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
@@ -594,7 +591,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             ++n_fixed;
           }
           ok = mbar_wait_warp(p_full, (g + j) & 1, a.status, s_abort) && ok;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             take();
             if (one) {
@@ -624,7 +621,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   } else if (E4M3 && warp >= 6) {
     // ------------------------------------------------ e4m3 codes to bf16, in place
     // Two warps per slot, four slots at a time, so that one team's waits lie beside the others' work. The
-    // codes come into the first half of the slot; a team takes them into registers, then writes all of it.
+    // TMA leaves the codes of key k where the second half of its bf16 row goes, so eight lanes that take a
+    // row's codes and then write both its halves need no other place, and no barrier but their warp's.
     const int t = threadIdx.x & 63;             // of the team's 64 threads
     const int team = (warp - 6) >> 1;           // the run's slots team, team + 4, ...
     const int key_lo = t >> 3, part = t & 7;    // keys key_lo + 8 u, 16 of 128 values
@@ -641,28 +639,33 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       uint8_t* base = ring + slot * kDcSlotBytes;
       ok = mbar_wait_warp(&raw[slot], phase, a.status, s_abort);
       if (blk < 4) {
-        const uint8_t* sc = smem + DcSmem::kScales + slot * 256 + blk;
-        uint4 w[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) w[u] = *reinterpret_cast<const uint4*>(base + (8 * u + key_lo) * 128 + part * 16);
-        named_bar_sync(2 + team, 64);  // all codes are in registers
-        // the next group's segment may be read meanwhile
+        const uint8_t* sc = smem + DcSmem::kScales + slot * 256 + blk + key_lo * 4;
         const int sure = max(0, grp.len - a.n_q + 1);
         bool bad = false;
         const int sw = part >> 2;
         uint8_t* row = base + sw * 8192 + key_lo * 128;
         // this thread's 32 bytes of chunk part / 4: the two halves in an order that keeps eight lanes on eight banks
         const uint32_t o0 = (uint32_t)((((part & 3) * 2 + sw) ^ key_lo) << 4), o1 = (uint32_t)((((part & 3) * 2 + 1 - sw) ^ key_lo) << 4);
-#pragma unroll
+        const uint8_t* src = base + 8192 + key_lo * 128 + part * 16;
+#pragma unroll 2
         for (int u = 0; u < 8; ++u) {
           const int key = first + 8 * u + key_lo;
-          uint32_t o[8];
-          if (key >= grp.len) w[u] = make_uint4(0u, 0u, 0u, 0u);
-          const bool nan = widen16(w[u], sc[(8 * u + key_lo) * 4], o);
-          bad |= nan && key >= sure;
-          const uint4 v0 = make_uint4(o[0], o[1], o[2], o[3]), v1 = make_uint4(o[4], o[5], o[6], o[7]);
-          *reinterpret_cast<uint4*>(row + u * 1024 + o0) = sw ? v1 : v0;
-          *reinterpret_cast<uint4*>(row + u * 1024 + o1) = sw ? v0 : v1;
+          uint2 q0 = *reinterpret_cast<const uint2*>(src + u * 1024 + 8 * sw);
+          uint2 q1 = *reinterpret_cast<const uint2*>(src + u * 1024 + 8 - 8 * sw);
+          const uint32_t e = sc[u * 32];
+          __syncwarp();
+          if (key >= grp.len) q0 = q1 = make_uint2(0u, 0u);
+          uint32_t v0[4], v1[4], nan = 0;
+          const uint32_t f = min(e + 120u, 254u) * 0x00800080u, f2 = (e - 7u) * 0x00800080u;
+          widen8(q0, f, e > 134u, f2, nan, v0);
+          widen8(q1, f, e > 134u, f2, nan, v1);
+          if (nan & 0x80808080u) {
+            nan8(q0, v0);
+            nan8(q1, v1);
+            bad |= key >= sure;
+          }
+          *reinterpret_cast<uint4*>(row + u * 1024 + o0) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
+          *reinterpret_cast<uint4*>(row + u * 1024 + o1) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
         }
         // values that some query may not see must not be NaN under its P = 0
         if (grp.v && __any_sync(0xffffffffu, bad) && lane < 2) {
