@@ -106,6 +106,13 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
     }
   }
 }
+// The same for two barriers.
+__device__ __forceinline__ bool mbar_wait2_warp(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* status,
+                                                volatile int* abort_flag) {
+  const bool ta = mbar_test(a, pa), tb = mbar_test(b, pb);
+  if (__all_sync(0xffffffffu, ta && tb)) return true;
+  return mbar_wait_warp(a, pa, status, abort_flag) && mbar_wait_warp(b, pb, status, abort_flag);
+}
 
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
@@ -136,12 +143,9 @@ __device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* ba
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-// Untiled bulk copy: both addresses and the size are multiples of 16.
-__device__ __forceinline__ void bulk_load(const void* src, uint64_t* bar, void* dst, uint32_t bytes) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
+// Brings global memory into L2 (address and size multiples of 16).
+__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
 // ---------------------------------------------------------------- cp.async (16-byte, L2 only)

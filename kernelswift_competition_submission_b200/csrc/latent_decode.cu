@@ -11,7 +11,7 @@
 //   warps 0-3  softmax: lane = row, warps 0-1 keys 0-63, warps 2-3 keys 64-127 of the tile; running
 //              maximum and sum, P into shared memory, O rescaled when the maximum has moved by 2^8
 //   warp 4     TMA producer: 16 KB slots ([64 keys][128 values]) in a ring of 8, in MMA order
-//   warps 6-13 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
+//   warps 6-21 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
 //              (exact: the scales are powers of two), two warps a slot
 //   warp 5     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
 //              beside PV of j - 1 and QK of j + 1
@@ -40,7 +40,8 @@ constexpr int kDcSlots = 8;
 constexpr int kDcSlotBytes = 16384;   // [64 keys][128 values]
 constexpr int kDcMaxPairs = 80;
 constexpr int kDcThreads = 192;       // 16-bit pages
-constexpr int kDcConv = 8;            // e4m3 pages: warps that widen the codes
+constexpr int kDcConv = 16;           // e4m3 pages: warps that widen the codes,
+constexpr int kDcTeam = 4;            // so many to a slot
 constexpr int kDcThreads8 = kDcThreads + 32 * kDcConv;
 constexpr float kDcRescaleLog2 = 8.0f;
 
@@ -48,8 +49,8 @@ struct DcSmem {
   static constexpr int kRing = 9 * 8192;                      // after Q: nine [64 rows][64] chunks
   static constexpr int kP = kRing + kDcSlots * kDcSlotBytes;  // two [64 rows][64 keys] chunks
   static constexpr int kX = kP + 16384;                       // row maxima / sums of both key halves, two tiles
-  static constexpr int kScales = kX + 2 * 128 * 4;            // e4m3: four scale bytes of a slot's 64 keys
-  static constexpr int kBars = kScales + kDcSlots * 256;
+  static constexpr int kScales = kX + 2 * 128 * 4;            // e4m3: four scale bytes of each of a slot's 64 keys, a copy (page) on 128 bytes
+  static constexpr int kBars = kScales + kDcSlots * 512;
   // full[8], empty[8], raw[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix, v_fixed
   static constexpr int kNumBars = 3 * kDcSlots + 10;
   static constexpr int kMisc = kBars + kNumBars * 8;
@@ -263,7 +264,8 @@ __device__ __forceinline__ void nan8(uint2 q, uint32_t (&o)[4]) {
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
 latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
-                     const __grid_constant__ CUtensorMap map_r, const __grid_constant__ DcArgs a) {
+                     const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_s,
+                     const __grid_constant__ DcArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + DcSmem::kRing;
@@ -323,7 +325,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
   }
   if (threadIdx.x == 32) {
-    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 4 : 1); mbar_init(&empty[s], 1); mbar_init(&raw[s], 1); }
+    for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 2 * kDcTeam : 1); mbar_init(&empty[s], 1); mbar_init(&raw[s], 1); }
     mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(&s_full[0], 1);
@@ -350,125 +352,114 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   DcSeg sg;
 
   if (warp == 4) {
-    // ------------------------------------------------ TMA producer
-    if (lane == 0) { tma_prefetch_desc(&map_q); tma_prefetch_desc(&map_c); }
+    // ------------------------------------------------ TMA producer: the warp converged, one lane issues, two
+    // slots at a time
     const bool one = elect_one();
     // one copy per slot when a page holds 64 keys, else one per page and 64 values
     const int br = min(a.page_size, 64), ppk = 64 / br;
     const uint32_t full0 = mapa_shared(full, 0);
-    int slot = 0, seg = 0;
-    uint32_t phase = 0, fix_phase = 0, issued = 0, issued_parity = 0;
+    uint32_t n = 0;  // slots of the run so far
+    int seg = 0;
+    uint32_t fix_phase = 0, issued = 0, issued_parity = 0;
     bool ok = true;
-    auto wait_empty = [&]() { return mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort); };
+    auto note = [&](uint32_t n) {
+      issued |= 1u << (n % kDcSlots);
+      issued_parity = (issued_parity & ~(1u << (n % kDcSlots))) | (((n / kDcSlots) & 1u) << (n % kDcSlots));
+    };
     // pages of a tile: lane l (l < 8) that of keys 16 l .. 16 l + 15
     auto pages_of = [&](const DcSeg& s, int j) {
       const int64_t pi = ((int64_t)j * kDcTile + (lane & 7) * 16) >> a.page_shift;
       return j < s.k1 && pi < a.table_width ? __ldg(a.table + s.b * a.ld_table + pi) : -1;
     };
-    auto copy_one = [&](int dst_off, int row, int ch, int page, bool local) {
-      uint8_t* dst = ring + slot * kDcSlotBytes + dst_off;
-      if (one) {
-        if (local) tma_load_4d(&map_c, fix, dst, 0, row, ch, page);
-        else tma_load_4d_pair(&map_c, full0 + slot * 8, dst, 0, row, ch, page);
-      }
-      __syncwarp();
-    };
-    // 64 keys (key half `half`) of tile j, 64-value chunks ch and ch + 1, into the slot. Chunk 9 does not
-    // exist and reads as zeros, so the rotary chunk's slot counts the same bytes. `local`: counted on
-    // this CTA's `fix`, else on the first CTA's `full`.
-    auto copy = [&](int pages, int half, int j, int ch, bool local) {
-      if (br == 64) {
-        copy_one(0, (j * kDcTile + half * 64) & (a.page_size - 1), ch, __shfl_sync(0xffffffffu, pages, half * 4), local);
-      } else {
-        for (int i = 0; i < ppk; ++i) {
-          const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
-          for (int d = 0; d < 2; ++d) copy_one(d * 8192 + i * br * 128, 0, ch + d, page, local);
-        }
-      }
-    };
-    // the first CTA's arrival expects both CTAs' bytes; the other's may be there before it
-    auto announce = [&](uint32_t bytes) {
-      if (rank == 0 && one) mbar_arrive_expect_tx(&full[slot], 2 * bytes);
-      __syncwarp();
-    };
-    // e4m3: 64 keys of tile j into the slot as they are, codes of value block blk with their scale bytes, or
-    // (blk 4) the rotary keys, which need no widening. Bytes are counted on this CTA's raw[slot].
-    auto copy_raw = [&](int pages, int half, int j, int blk) {
-      uint8_t* dst = ring + slot * kDcSlotBytes + (blk < 4 ? 8192 : 0);
-      uint8_t* sdst = smem + DcSmem::kScales + slot * 256;
+    // One slot, by the elected lane: 64 keys of tile j (from key half `half`; pg: their pages, by copy), value
+    // block blk of 128 (4: the rotary keys). 16-bit pages: counted on the first CTA's `full` (whose own
+    // arrival expects both CTAs' bytes), or with `local` on this CTA's `fix`; chunk 9 does not exist and reads
+    // as zeros, so the rotary slot counts the same bytes. e4m3 pages: as they are, counted on this CTA's raw[]:
+    // codes into the second half of the slot, their scale bytes aside, rotary keys in place.
+    auto copy = [&](uint32_t n, const int (&pg)[4], int half, int j, int blk, bool local) {
+      const int sl = n % kDcSlots;
+      uint8_t* dst = ring + sl * kDcSlotBytes;
       const int row = br == 64 ? (j * kDcTile + half * 64) & (a.page_size - 1) : 0;
-      uint32_t bytes = 8192;
-      if (blk < 4)
+      if constexpr (E4M3) {
+        mbar_arrive_expect_tx(&raw[sl], blk < 4 ? 8192 + 256 : 8192);
         for (int i = 0; i < ppk; ++i) {
-          const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
-          if (page >= 0 && page < a.num_pages) bytes += br * 4;  // a page outside the cache has no scales
-        }
-      if (one) mbar_arrive_expect_tx(&raw[slot], bytes);
-      for (int i = 0; i < ppk; ++i) {
-        const int page = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4));
-        if (one) {
           if (blk < 4) {
-            tma_load_3d(&map_c, &raw[slot], dst + i * br * 128, blk * 128, row, page);
-            if (page >= 0 && page < a.num_pages)
-              bulk_load(a.cache + (int64_t)page * (a.page_size * kRow8Bytes) + a.page_size * (kLatDim + 2 * kRopeDim) + row * 4,
-                        &raw[slot], sdst + i * br * 4, br * 4);
+            tma_load_3d(&map_c, &raw[sl], dst + 8192 + i * br * 128, blk * 128, row, pg[i]);
+            tma_load_3d(&map_s, &raw[sl], smem + DcSmem::kScales + sl * 512 + i * max(br * 4, 128), row * 4, 0, pg[i]);
           } else {
-            tma_load_3d(&map_r, &raw[slot], dst + i * br * 128, 0, row, page);
+            tma_load_3d(&map_r, &raw[sl], dst + i * br * 128, 0, row, pg[i]);
           }
         }
-        __syncwarp();
+      } else {
+        if (!local && rank == 0) mbar_arrive_expect_tx(&full[sl], 2 * kDcSlotBytes);
+        if (br == 64) {
+          if (local) tma_load_4d(&map_c, fix, dst, 0, row, blk * 2, pg[0]);
+          else tma_load_4d_pair(&map_c, full0 + sl * 8, dst, 0, row, blk * 2, pg[0]);
+        } else {
+          for (int i = 0; i < 2 * ppk; ++i) {
+            uint8_t* d = dst + (i & 1) * 8192 + (i >> 1) * br * 128;
+            if (local) tma_load_4d(&map_c, fix, d, 0, 0, blk * 2 + (i & 1), pg[i >> 1]);
+            else tma_load_4d_pair(&map_c, full0 + sl * 8, d, 0, 0, blk * 2 + (i & 1), pg[i >> 1]);
+          }
+        }
       }
     };
-    auto step = [&]() {
-      issued |= 1u << slot;
-      issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
-      if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
+    auto half_pages = [&](int pages, int half, int (&pg)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4 & 3));
+    };
+    auto wait_two = [&](uint32_t n) {
+      return mbar_wait2_warp(&empty[n % kDcSlots], ((n / kDcSlots) & 1u) ^ 1u, &empty[(n + 1) % kDcSlots],
+                             (((n + 1) / kDcSlots) & 1u) ^ 1u, a.status, s_abort);
     };
     auto load_k = [&](int pages, int j) {
-      for (int c = 0; c < 5; ++c) {
-        if (!wait_empty()) return false;
-        if constexpr (E4M3) {
-          copy_raw(pages, (int)rank, j, c);
-        } else {
-          announce(kDcSlotBytes);
-          copy(pages, (int)rank, j, c * 2, false);
+      int pg[4];
+      half_pages(pages, (int)rank, pg);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        if (!wait_two(n + c)) return false;
+        if (one) {
+          copy(n + c, pg, (int)rank, j, c, false);
+          copy(n + c + 1, pg, (int)rank, j, c + 1, false);
         }
-        step();
+        __syncwarp();
+        note(n + c);
+        note(n + c + 1);
       }
+      if (!mbar_wait_warp(&empty[(n + 4) % kDcSlots], (((n + 4) / kDcSlots) & 1u) ^ 1u, a.status, s_abort)) return false;
+      if (one) copy(n + 4, pg, (int)rank, j, 4, false);
+      __syncwarp();
+      note(n + 4);
+      n += 5;
       return true;
     };
+    // slot order of V: value block 0 keys 0-63, 64-127, value block 1 keys 0-63, 64-127
     auto load_v = [&](const DcSeg& s, int pages, int j) {
-      // slot order: value block 0 keys 0-63, 64-127, value block 1 keys 0-63, 64-127
+      int pg0[4], pg1[4];
+      half_pages(pages, 0, pg0);
+      half_pages(pages, 1, pg1);
       const int sure = max(0, s.len - a.n_q + 1);  // keys that every row sees
-      if (E4M3 || (j + 1) * kDcTile <= sure) {
-        for (int c = 0; c < 4; ++c) {
-          if (!wait_empty()) return false;
-          if constexpr (E4M3) {
-            copy_raw(pages, c & 1, j, (c >> 1) * 2 + (int)rank);
-          } else {
-            announce(kDcSlotBytes);
-            copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, false);
-          }
-          step();
+      const bool local = !E4M3 && (j + 1) * kDcTile > sure;
+      if (local && one) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        if (!wait_two(n + c)) return false;
+        if (one) {
+          copy(n + c, pg0, 0, j, c + (int)rank, local);
+          copy(n + c + 1, pg1, 1, j, c + (int)rank, local);
         }
-        return true;
-      }
-      // some row does not see all of this tile: bring V in on this CTA's own barrier, zero the rows
-      // past the length, look at the rows some query may not see, then hand the slots over
-      const int slot0 = slot;
-      const uint32_t phase0 = phase;
-      for (int c = 0; c < 4; ++c) {
-        if (!wait_empty()) return false;
-        if (c == 0 && one) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
         __syncwarp();
-        copy(pages, c & 1, j, (c >> 1) * 4 + (int)rank * 2, true);
-        step();
+        if (!local) { note(n + c); note(n + c + 1); }
       }
+      n += 4;
+      if (!local) return true;
+      // some row does not see all of this tile: V came in on this CTA's own barrier; zero the rows past the
+      // length, look at the rows some query may not see, then hand the slots over
       if (!mbar_wait_warp(fix, fix_phase, a.status, s_abort)) return false;
       fix_phase ^= 1;
       uint32_t worst = 0;
       for (int c = 0; c < 4; ++c) {
-        uint8_t* base = ring + ((slot0 + c) % kDcSlots) * kDcSlotBytes;
+        uint8_t* base = ring + ((n - 4 + c) % kDcSlots) * kDcSlotBytes;
         const int key0 = j * kDcTile + (c & 1) * 64;
         for (int v = max(0, sure - key0) * 16 + lane; v < 64 * 16; v += 32) {  // 16-byte pieces of rows >= sure
           const int row = v >> 4;
@@ -489,21 +480,12 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (rank != 0) {
-        if (one) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
-        __syncwarp();
-        return true;
+      if (one) {
+        if (rank != 0) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
+        else
+          for (int c = 0; c < 4; ++c) mbar_arrive(&full[(n - 4 + c) % kDcSlots]);
       }
-      const int slot1 = slot;
-      const uint32_t phase1 = phase;
-      slot = slot0;
-      phase = phase0;
-      for (int c = 0; c < 4; ++c) {
-        announce(0);
-        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
-      }
-      slot = slot1;
-      phase = phase1;
+      __syncwarp();
       return true;
     };
     while (ok && it.next(a, sg)) {
@@ -620,52 +602,75 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     }
   } else if (E4M3 && warp >= 6) {
     // ------------------------------------------------ e4m3 codes to bf16, in place
-    // Two warps per slot, four slots at a time, so that one team's waits lie beside the others' work. The
-    // TMA leaves the codes of key k where the second half of its bf16 row goes, so eight lanes that take a
-    // row's codes and then write both its halves need no other place, and no barrier but their warp's.
-    const int t = threadIdx.x & 63;             // of the team's 64 threads
-    const int team = (warp - 6) >> 1;           // the run's slots team, team + 4, ...
-    const int key_lo = t >> 3, part = t & 7;    // keys key_lo + 8 u, 16 of 128 values
+    // kDcTeam warps per slot and several slots at a time, so that one slot's waits lie beside the others'
+    // work. The TMA leaves the codes of key k where the second half of its bf16 row goes, so eight lanes that
+    // take a row's codes and then write both its halves need no other place, and no barrier but their warp's.
+    constexpr int kTeams = kDcConv / kDcTeam, kStride = 4 * kDcTeam;   // keys per round of a team
+    static_assert(kStride == 16, "a round is one page's keys where pages hold 16");
+    const int t = threadIdx.x - kDcThreads;
+    const int key_lo = (t >> 3) % kStride, part = t & 7;               // keys key_lo + kStride u, 16 of 128 values
+    int slot = (warp - 6) / kDcTeam;                                   // the run's slots team, team + kTeams, ...
     const uint32_t full0 = mapa_shared(full, 0);
     DcGroups gen{it, {}, 0, 0, 0, 0, -1};
-    DcGroup grp;
-    int c = team, slot = team;                  // slot of the tile's K or V, and of the ring
+    DcGroup grp{};
+    int c = slot;                                                      // slot of the tile's K or V
     uint32_t phase = 0;
-    bool ok = true;
-    bool more = gen.next(a, grp);
+    bool ok = true, more = true;
+    auto settle = [&]() {  // c counts from the group: move on to the group that holds it
+      while (more && c >= (grp.v ? 4 : 5)) {
+        c -= grp.v ? 4 : 5;
+        more = gen.next(a, grp);
+      }
+    };
+    more = gen.next(a, grp);
+    settle();
     while (more && ok) {
       const int half = grp.v ? (c & 1) : (int)rank, blk = grp.v ? 2 * (c >> 1) + (int)rank : c;
       const int first = grp.j * kDcTile + half * 64;
       uint8_t* base = ring + slot * kDcSlotBytes;
       ok = mbar_wait_warp(&raw[slot], phase, a.status, s_abort);
       if (blk < 4) {
-        const uint8_t* sc = smem + DcSmem::kScales + slot * 256 + blk + key_lo * 4;
+        // TMA writes start on 128 bytes: with pages of 16 keys a page's 64 scale bytes are that far apart
+        const uint8_t* sc = smem + DcSmem::kScales + slot * 512 + blk + key_lo * 4;
+        const int sc_step = a.page_size == 16 ? kStride / 16 * 128 : kStride * 4;
         const int sure = max(0, grp.len - a.n_q + 1);
         bool bad = false;
-        const int sw = part >> 2;
+        const int sw = part >> 2, x = key_lo & 7;
         uint8_t* row = base + sw * 8192 + key_lo * 128;
         // this thread's 32 bytes of chunk part / 4: the two halves in an order that keeps eight lanes on eight banks
-        const uint32_t o0 = (uint32_t)((((part & 3) * 2 + sw) ^ key_lo) << 4), o1 = (uint32_t)((((part & 3) * 2 + 1 - sw) ^ key_lo) << 4);
+        const uint32_t o0 = (uint32_t)((((part & 3) * 2 + sw) ^ x) << 4), o1 = (uint32_t)((((part & 3) * 2 + 1 - sw) ^ x) << 4);
         const uint8_t* src = base + 8192 + key_lo * 128 + part * 16;
-#pragma unroll 2
-        for (int u = 0; u < 8; ++u) {
-          const int key = first + 8 * u + key_lo;
-          uint2 q0 = *reinterpret_cast<const uint2*>(src + u * 1024 + 8 * sw);
-          uint2 q1 = *reinterpret_cast<const uint2*>(src + u * 1024 + 8 - 8 * sw);
-          const uint32_t e = sc[u * 32];
-          __syncwarp();
-          if (key >= grp.len) q0 = q1 = make_uint2(0u, 0u);
-          uint32_t v0[4], v1[4], nan = 0;
-          const uint32_t f = min(e + 120u, 254u) * 0x00800080u, f2 = (e - 7u) * 0x00800080u;
-          widen8(q0, f, e > 134u, f2, nan, v0);
-          widen8(q1, f, e > 134u, f2, nan, v1);
-          if (nan & 0x80808080u) {
-            nan8(q0, v0);
-            nan8(q1, v1);
-            bad |= key >= sure;
+        constexpr int kU = 2;  // keys at a time
+#pragma unroll 1
+        for (int u = 0; u < 64 / kStride; u += kU) {
+          uint32_t v0[kU][4], v1[kU][4];
+          uint2 q0[kU], q1[kU];
+          uint32_t e[kU];
+#pragma unroll
+          for (int i = 0; i < kU; ++i) {
+            q0[i] = *reinterpret_cast<const uint2*>(src + (u + i) * (kStride * 128) + 8 * sw);
+            q1[i] = *reinterpret_cast<const uint2*>(src + (u + i) * (kStride * 128) + 8 - 8 * sw);
+            e[i] = sc[(u + i) * sc_step];
+            if (first + kStride * (u + i) + key_lo >= grp.len) q0[i] = q1[i] = make_uint2(0u, 0u);
           }
-          *reinterpret_cast<uint4*>(row + u * 1024 + o0) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
-          *reinterpret_cast<uint4*>(row + u * 1024 + o1) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
+#pragma unroll
+          for (int i = 0; i < kU; ++i) {
+            uint32_t nan = 0;
+            const uint32_t f = min(e[i] + 120u, 254u) * 0x00800080u, f2 = (e[i] - 7u) * 0x00800080u;
+            widen8(q0[i], f, e[i] > 134u, f2, nan, v0[i]);
+            widen8(q1[i], f, e[i] > 134u, f2, nan, v1[i]);
+            if (nan & 0x80808080u) {
+              nan8(q0[i], v0[i]);
+              nan8(q1[i], v1[i]);
+              bad |= first + kStride * (u + i) + key_lo >= sure;
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < kU; ++i) {
+            *reinterpret_cast<uint4*>(row + (u + i) * (kStride * 128) + o0) = make_uint4(v0[i][0], v0[i][1], v0[i][2], v0[i][3]);
+            *reinterpret_cast<uint4*>(row + (u + i) * (kStride * 128) + o1) = make_uint4(v1[i][0], v1[i][1], v1[i][2], v1[i][3]);
+          }
         }
         // values that some query may not see must not be NaN under its P = 0
         if (grp.v && __any_sync(0xffffffffu, bad) && lane < 2) {
@@ -676,14 +681,10 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
-      slot ^= 4;  // the team's other slot of the ring
-      if (slot < 4) phase ^= 1;
-      c += 4;
-      const int n = grp.v ? 4 : 5;
-      if (c >= n) {
-        c -= n;
-        more = gen.next(a, grp);
-      }
+      slot += kTeams;
+      if (slot >= kDcSlots) { slot -= kDcSlots; phase ^= 1; }
+      c += kTeams;
+      settle();
     }
   } else {
     // ------------------------------------------------ softmax
@@ -717,41 +718,43 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         // a wait that gave up is carried to the next barrier of the four warps, so that all leave together
         ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
         tc_fence_after();
-        uint32_t raw[2][32];
-        tmem_ld32(lane_base + kTmemS + (g & 1) * 64, raw[0]);
-        tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + 32, raw[1]);
-        tmem_wait_ld();
-        if (a.neg) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int x = 0; x < 32; ++x) raw[c][x] ^= 0x80000000u;
-        }
+        // 32 scores at a time, read twice from TMEM (maximum, then exponentials): 64 in registers beside
+        // P would not leave room for the warps that widen codes
         const int key0 = j * kDcTile + half * 64;
         const int vis = limit - key0;
-        if (__any_sync(0xffffffffu, vis < 64)) {
+        const bool partly = __any_sync(0xffffffffu, vis < 64);
+        auto scores = [&](int c, uint32_t (&raw)[32]) {
+          tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + c * 32, raw);
+          tmem_wait_ld();
+          if (a.neg) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int x = 0; x < 32; ++x) raw[x] ^= 0x80000000u;
+          }
+          if (partly) {
 #pragma unroll
             for (int x = 0; x < 32; ++x)
-              if (c * 32 + x >= vis) raw[c][x] = 0xFF800000u;
-        }
-        if (bad_page) {
+              if (c * 32 + x >= vis) raw[x] = 0xFF800000u;
+          }
+          if (bad_page) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int64_t pi = ((int64_t)key0 + u * 16) >> a.page_shift;
-            const int v = pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
-            if (v < 0 || v >= a.num_pages) {
+            for (int u = 0; u < 2; ++u) {
+              const int64_t pi = ((int64_t)key0 + c * 32 + u * 16) >> a.page_shift;
+              const int v = pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
+              if (v < 0 || v >= a.num_pages) {
 #pragma unroll
-              for (int x = 0; x < 16; ++x) raw[u >> 1][(u & 1) * 16 + x] = 0xFF800000u;
+                for (int x = 0; x < 16; ++x) raw[u * 16 + x] = 0xFF800000u;
+              }
             }
           }
-        }
+        };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32];
+          scores(c, raw);
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[c][x]));
+          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[x]));
+        }
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // the row's other 64 keys are with the thread 64 further on
         float* x = s_x + (g & 1) * 128;
@@ -770,12 +773,17 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t p[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float p0 = ex2d(fmaf(__uint_as_float(raw[e >> 4][(2 * e) & 31]), a.scale_log2, -base));
-          const float p1 = ex2d(fmaf(__uint_as_float(raw[e >> 4][((2 * e) & 31) + 1]), a.scale_log2, -base));
-          sum[e & 1] += p0;
-          sum[2 + (e & 1)] += p1;
-          p[e] = ElemTraits<T>::pack2(p0, p1);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t raw[32];
+          scores(c, raw);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = ex2d(fmaf(__uint_as_float(raw[2 * e]), a.scale_log2, -base));
+            const float p1 = ex2d(fmaf(__uint_as_float(raw[2 * e + 1]), a.scale_log2, -base));
+            sum[e & 1] += p0;
+            sum[2 + (e & 1)] += p1;
+            p[c * 16 + e] = ElemTraits<T>::pack2(p0, p1);
+          }
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (j > sg.k0) {  // PV of the tile before: its P is read, its O is written
@@ -986,7 +994,7 @@ cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
 
 template <typename T, bool E4M3>
 cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
-  CUtensorMap mq, mc, mr;
+  CUtensorMap mq, mc, mr, ms;
   const uint64_t row = 2 * kRowDim;
   const uint64_t dq[4] = {64, (uint64_t)a.rows, kRowDim / 64, (uint64_t)a.num_seqs};
   const uint64_t sq[3] = {row, 128, row * (uint64_t)a.rows};
@@ -996,13 +1004,16 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   if (E4M3) {
     const uint64_t dc[3] = {kLatDim, (uint64_t)a.page_size, (uint64_t)a.num_pages}, sc[2] = {kLatDim, page8};
     const uint64_t dr[3] = {kRopeDim, (uint64_t)a.page_size, (uint64_t)a.num_pages}, sr[2] = {2 * kRopeDim, page8};
-    maps = maps && make_bytes_map(&mc, a.cache, dc, sc, box_rows) &&
+    const uint64_t scale_row = (uint64_t)a.page_size * 4;  // a page's scale bytes
+    const uint64_t ds[3] = {scale_row, 1, (uint64_t)a.num_pages}, ss[2] = {scale_row, page8};
+    maps = maps && make_bytes_map(&mc, a.cache, dc, sc, box_rows, 128) &&
+           make_bytes_map(&ms, a.cache + (size_t)a.page_size * (kLatDim + 2 * kRopeDim), ds, ss, 1, box_rows * 4) &&
            make_kmajor_map(&mr, dtype, a.cache + (size_t)a.page_size * kLatDim, 3, dr, sr, box_rows);
   } else {
     const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
     const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
     maps = maps && make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1);
-    mr = mc;
+    mr = ms = mc;
   }
   if (!maps) return cudaErrorInvalidValue;
   auto kern = latent_decode_kernel<T, E4M3>;
@@ -1021,7 +1032,7 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   cfg.numAttrs = 1;
   if ((err = resident_pairs(kern, cfg, &a.pairs)) != cudaSuccess) return err;
   cfg.gridDim = dim3(2 * (unsigned)a.pairs, 1, 1);
-  if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, mr, a)) != cudaSuccess) return err;
+  if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, mr, ms, a)) != cudaSuccess) return err;
   latent_decode_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.num_seqs * a.rows, 4), 128, 0, st>>>(a);
   return cudaGetLastError();
 }

@@ -95,7 +95,7 @@ bool make_chunks_map(CUtensorMap* m, int dtype, const void* base, const uint64_t
                      uint32_t box_rows, uint32_t box_chunks);
 
 bool make_bytes_map(CUtensorMap* m, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
-                    uint32_t box_rows);
+                    uint32_t box_rows, uint32_t box_bytes);
 
 bool make_fp8_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                   uint32_t box_rows);

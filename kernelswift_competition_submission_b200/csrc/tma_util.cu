@@ -158,15 +158,16 @@ bool make_fp8_map(CUtensorMap* m, const void* base, int rank, const uint64_t* di
   return true;
 }
 
-// Byte map of rank 3, no swizzle: boxes of [box_rows][128 bytes].
+// Byte map of rank 3, no swizzle: boxes of [box_rows][box_bytes].
 bool make_bytes_map(CUtensorMap* m, const void* base, const uint64_t* dims, const uint64_t* strides_bytes,
-                    uint32_t box_rows) {
-  const MapKey key = map_key(kMapBytes, 0, base, 3, dims, strides_bytes, box_rows);
+                    uint32_t box_rows, uint32_t box_bytes) {
+  MapKey key = map_key(kMapBytes, 0, base, 3, dims, strides_bytes, box_rows);
+  key.box_outer = box_bytes;
   if (cache_lookup(key, m)) return true;
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return false;
   cuuint64_t gdim[3], gstr[2] = {strides_bytes[0], strides_bytes[1]};
-  cuuint32_t box[3] = {128, box_rows, 1}, estr[3] = {1, 1, 1};
+  cuuint32_t box[3] = {box_bytes, box_rows, 1}, estr[3] = {1, 1, 1};
   for (int i = 0; i < 3; ++i) gdim[i] = dims[i];
   if (enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), gdim, gstr, box, estr,
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
