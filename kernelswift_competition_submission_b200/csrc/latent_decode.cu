@@ -8,12 +8,14 @@
 // sums fill 256 of its 512 TMEM columns (a single CTA with 128 rows would need all of them and have
 // no place for the scores). For S = Q K^T each CTA supplies 64 of the 128 keys, for O += P V it
 // supplies half of V's columns, so a key's row crosses from L2 to shared memory twice per pair.
-//   warps 0-3  softmax: lane = row, warps 0-1 keys 0-63, warps 2-3 keys 64-127 of the tile; running
-//              maximum and sum, P into shared memory, O rescaled when the maximum has moved by 2^8
-//   warp 4     TMA producer: 16 KB slots ([64 keys][128 values]) in a ring of 8, in MMA order
-//   warps 6-21 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
+//   warps 0-7  softmax: four threads per row with 32 keys each (TMEM gives a warp 32 of the 128 lanes; lanes
+//              0-63 hold keys 0-63, lanes 64-127 keys 64-127); running maximum and sum, P into shared memory, O
+//              rescaled when the maximum has moved by 2^8
+//   warps 8, 10 TMA producers of K and of V: 16 KB slots ([64 keys][128 values]), four for a tile's K and four for
+//              its V, the rotary keys in a buffer of their own; each slot is refilled as soon as it has been read
+//   warps 11-26 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
 //              (exact: the scales are powers of two), two warps a slot
-//   warp 5     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
+//   warp 9     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
 //              beside PV of j - 1 and QK of j + 1
 //
 // The (request, row tile, key tile) list is cut into equal runs, one per pair, by lengths read on
@@ -39,20 +41,22 @@ constexpr int kDcRows = 64;           // rows per CTA
 constexpr int kDcSlots = 8;
 constexpr int kDcSlotBytes = 16384;   // [64 keys][128 values]
 constexpr int kDcMaxPairs = 80;
-constexpr int kDcThreads = 192;       // 16-bit pages
+constexpr int kDcSoftmax = 256;       // threads of the softmax warps
+constexpr int kDcThreads = kDcSoftmax + 96;  // 16-bit pages
 constexpr int kDcConv = 16;           // e4m3 pages: warps that widen the codes,
-constexpr int kDcTeam = 4;            // so many to a slot
+constexpr int kDcTeam = 8;            // so many to a slot
 constexpr int kDcThreads8 = kDcThreads + 32 * kDcConv;
 constexpr float kDcRescaleLog2 = 8.0f;
 
 struct DcSmem {
   static constexpr int kRing = 9 * 8192;                      // after Q: nine [64 rows][64] chunks
-  static constexpr int kP = kRing + kDcSlots * kDcSlotBytes;  // two [64 rows][64 keys] chunks
-  static constexpr int kX = kP + 16384;                       // row maxima / sums of both key halves, two tiles
-  static constexpr int kScales = kX + 2 * 128 * 4;            // e4m3: four scale bytes of each of a slot's 64 keys, a copy (page) on 128 bytes
-  static constexpr int kBars = kScales + kDcSlots * 512;
-  // full[8], empty[8], raw[8], q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done, fix, v_fixed
-  static constexpr int kNumBars = 3 * kDcSlots + 10;
+  static constexpr int kRope = kRing + kDcSlots * kDcSlotBytes;  // [64 keys][64]
+  static constexpr int kP = kRope + 8192;                     // two [64 rows][64 keys] chunks
+  static constexpr int kX = kP + 16384;                       // the row's threads' maxima (bf16, two tiles) or sums
+  static constexpr int kBars = kX + kDcSoftmax * 4;
+  // full[8], empty[8], raw[8], rope_full, rope_free, q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done,
+  // fix, v_fixed
+  static constexpr int kNumBars = 3 * kDcSlots + 12;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kBytes = kMisc + 64 + 1024;
 };
@@ -212,28 +216,6 @@ __device__ __noinline__ void decode_row(const DcArgs& a, int b, int r, int kb, i
 }
 
 // ---------------------------------------------------------------- e4m3 pages into 16-bit slots
-// The slots of one tile in MMA order: K0 K1 V0 K2 V1 ... over the run's segments.
-struct DcGroup {
-  int b, j, len, v;  // request, key tile, positions held; v: V (four slots), else K (five)
-};
-struct DcGroups {
-  DcIter it;
-  DcSeg sg;
-  int i, nt, next_k, next_v, seg;
-  __device__ __forceinline__ bool next(const DcArgs& a, DcGroup& g) {
-    if (next_v >= nt) {
-      if (!it.next(a, sg)) return false;
-      nt = sg.k1 - sg.k0;
-      next_k = next_v = 0;
-      ++seg;
-    }
-    g.b = sg.b;
-    g.len = sg.len;
-    g.v = next_k >= nt || next_k >= next_v + 2;
-    g.j = sg.k0 + (g.v ? next_v++ : next_k++);
-    return true;
-  }
-};
 // 8 codes times 2^(e - 127) as bf16: f is bf16 2^min(e - 7, 127) in both halves, f2 what is left of it
 // (e above 134 only). The codes' exponent and fraction moved to the low end of bf16's are the value times
 // 2^-120, subnormals included, and the multiply rounds nothing. Bit 7 of a byte of `nan`: a NaN code, which
@@ -272,15 +254,17 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   uint8_t* s_p = smem + DcSmem::kP;
   float* s_x = reinterpret_cast<float*>(smem + DcSmem::kX);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + DcSmem::kBars);
-  uint64_t* full = bars;                 // first CTA's: both CTAs' copies of a slot
+  uint64_t* full = bars;                 // first CTA's: both CTAs' copies of a slot (0-3: K, 4-7: V)
   uint64_t* empty = full + kDcSlots;     // each CTA's
   uint64_t* raw = empty + kDcSlots;      // each CTA's, e4m3: codes and scales of a slot
-  uint64_t* q_full = raw + kDcSlots;     // first CTA's
+  uint64_t* rope_full = raw + kDcSlots;  // first CTA's
+  uint64_t* rope_free = rope_full + 1;   // each CTA's
+  uint64_t* q_full = rope_free + 1;      // first CTA's
   uint64_t* q_free = q_full + 1;
   uint64_t* s_full = q_free + 1;         // [2]
-  uint64_t* p_full = s_full + 2;         // first CTA's: eight softmax warps
+  uint64_t* p_full = s_full + 2;         // first CTA's: both CTAs' softmax warps
   uint64_t* pv_done = p_full + 1;
-  uint64_t* o_free = pv_done + 1;        // first CTA's: eight softmax warps
+  uint64_t* o_free = pv_done + 1;        // first CTA's: both CTAs' softmax warps
   uint64_t* mma_done = o_free + 1;
   uint64_t* fix = mma_done + 1;
   uint64_t* v_fixed = fix + 1;           // first CTA's: the other CTA has looked at its V
@@ -326,13 +310,15 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   }
   if (threadIdx.x == 32) {
     for (int s = 0; s < kDcSlots; ++s) { mbar_init(&full[s], E4M3 ? 2 * kDcTeam : 1); mbar_init(&empty[s], 1); mbar_init(&raw[s], 1); }
+    mbar_init(rope_full, 1);
+    mbar_init(rope_free, 1);
     mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(p_full, 8);
+    mbar_init(p_full, 2 * kDcSoftmax / 32);
     mbar_init(pv_done, 1);
-    mbar_init(o_free, 8);
+    mbar_init(o_free, 2 * kDcSoftmax / 32);
     mbar_init(mma_done, 1);
     mbar_init(fix, 1);
     mbar_init(v_fixed, 1);
@@ -341,7 +327,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     *s_badpage = 0;
     fence_mbar_init();
   }
-  if (warp == 5) { tmem_alloc_pair(s_tmem, 512); tmem_relinquish_pair(); }
+  if (warp == 9) { tmem_alloc_pair(s_tmem, 512); tmem_relinquish_pair(); }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // barriers of both CTAs are ready
@@ -349,46 +335,37 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   const uint32_t tmem = *s_tmem;
   constexpr uint32_t kTmemS = 256;  // O: columns 0-127 and 128-255, S: 256-319 and 320-383
   DcIter it{s_plan[0], *reinterpret_cast<int64_t*>(s_plan + 2), *reinterpret_cast<int64_t*>(s_plan + 4)};
-  DcSeg sg;
+  DcSeg sg{};
 
-  if (warp == 4) {
-    // ------------------------------------------------ TMA producer: the warp converged, one lane issues, two
+  if (warp == 8 || warp == 10) {
+    // ------------------------------------------------ TMA producers: the warp converged, one lane issues, two
     // slots at a time
     const bool one = elect_one();
+    const bool for_v = warp == 10;
+    const int slot0 = for_v ? 4 : 0;
     // one copy per slot when a page holds 64 keys, else one per page and 64 values
     const int br = min(a.page_size, 64), ppk = 64 / br;
     const uint32_t full0 = mapa_shared(full, 0);
-    uint32_t n = 0;  // slots of the run so far
     int seg = 0;
-    uint32_t fix_phase = 0, issued = 0, issued_parity = 0;
+    uint32_t g = 0, fix_phase = 0;  // g: tiles of the run so far
     bool ok = true;
-    auto note = [&](uint32_t n) {
-      issued |= 1u << (n % kDcSlots);
-      issued_parity = (issued_parity & ~(1u << (n % kDcSlots))) | (((n / kDcSlots) & 1u) << (n % kDcSlots));
-    };
     // pages of a tile: lane l (l < 8) that of keys 16 l .. 16 l + 15
-    auto pages_of = [&](const DcSeg& s, int j) {
+    auto pages_of = [&](int j) {
       const int64_t pi = ((int64_t)j * kDcTile + (lane & 7) * 16) >> a.page_shift;
-      return j < s.k1 && pi < a.table_width ? __ldg(a.table + s.b * a.ld_table + pi) : -1;
+      return j < sg.k1 && pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
     };
     // One slot, by the elected lane: 64 keys of tile j (from key half `half`; pg: their pages, by copy), value
-    // block blk of 128 (4: the rotary keys). 16-bit pages: counted on the first CTA's `full` (whose own
-    // arrival expects both CTAs' bytes), or with `local` on this CTA's `fix`; chunk 9 does not exist and reads
-    // as zeros, so the rotary slot counts the same bytes. e4m3 pages: as they are, counted on this CTA's raw[]:
-    // codes into the second half of the slot, their scale bytes aside, rotary keys in place.
-    auto copy = [&](uint32_t n, const int (&pg)[4], int half, int j, int blk, bool local) {
-      const int sl = n % kDcSlots;
+    // block blk of 128. 16-bit pages: counted on the first CTA's `full` (whose own arrival expects both CTAs'
+    // bytes), or with `local` on this CTA's `fix`. e4m3 pages: as they are, counted on this CTA's raw[], the codes
+    // into the second half of the slot, their scale bytes into the first.
+    auto copy = [&](int sl, const int (&pg)[4], int half, int j, int blk, bool local) {
       uint8_t* dst = ring + sl * kDcSlotBytes;
       const int row = br == 64 ? (j * kDcTile + half * 64) & (a.page_size - 1) : 0;
       if constexpr (E4M3) {
-        mbar_arrive_expect_tx(&raw[sl], blk < 4 ? 8192 + 256 : 8192);
+        mbar_arrive_expect_tx(&raw[sl], 8192 + 256);
         for (int i = 0; i < ppk; ++i) {
-          if (blk < 4) {
-            tma_load_3d(&map_c, &raw[sl], dst + 8192 + i * br * 128, blk * 128, row, pg[i]);
-            tma_load_3d(&map_s, &raw[sl], smem + DcSmem::kScales + sl * 512 + i * max(br * 4, 128), row * 4, 0, pg[i]);
-          } else {
-            tma_load_3d(&map_r, &raw[sl], dst + i * br * 128, 0, row, pg[i]);
-          }
+          tma_load_3d(&map_c, &raw[sl], dst + 8192 + i * br * 128, blk * 128, row, pg[i]);
+          tma_load_3d(&map_s, &raw[sl], dst + i * max(br * 4, 128), row * 4, 0, pg[i]);
         }
       } else {
         if (!local && rank == 0) mbar_arrive_expect_tx(&full[sl], 2 * kDcSlotBytes);
@@ -408,50 +385,50 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 #pragma unroll
       for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4 & 3));
     };
-    auto wait_two = [&](uint32_t n) {
-      return mbar_wait2_warp(&empty[n % kDcSlots], ((n / kDcSlots) & 1u) ^ 1u, &empty[(n + 1) % kDcSlots],
-                             (((n + 1) / kDcSlots) & 1u) ^ 1u, a.status, s_abort);
+    auto wait_two = [&](int c) {  // slots c, c + 1 of this warp's four have been read
+      return mbar_wait_lanes(lane < 2 ? &empty[slot0 + c + lane] : nullptr, (g & 1u) ^ 1u, a.status, s_abort);
     };
     auto load_k = [&](int pages, int j) {
       int pg[4];
       half_pages(pages, (int)rank, pg);
 #pragma unroll 1
       for (int c = 0; c < 4; c += 2) {
-        if (!wait_two(n + c)) return false;
+        if (!wait_two(c)) return false;
         if (one) {
-          copy(n + c, pg, (int)rank, j, c, false);
-          copy(n + c + 1, pg, (int)rank, j, c + 1, false);
+          copy(c, pg, (int)rank, j, c, false);
+          copy(c + 1, pg, (int)rank, j, c + 1, false);
         }
         __syncwarp();
-        note(n + c);
-        note(n + c + 1);
       }
-      if (!mbar_wait_warp(&empty[(n + 4) % kDcSlots], (((n + 4) / kDcSlots) & 1u) ^ 1u, a.status, s_abort)) return false;
-      if (one) copy(n + 4, pg, (int)rank, j, 4, false);
+      if (!mbar_wait_warp(rope_free, (g & 1u) ^ 1u, a.status, s_abort)) return false;
+      if (one) {
+        const int row = br == 64 ? (j * kDcTile + (int)rank * 64) & (a.page_size - 1) : 0;
+        if (rank == 0) mbar_arrive_expect_tx(rope_full, 2 * 8192);
+        for (int i = 0; i < ppk; ++i)
+          tma_load_3d_pair(&map_r, full0 + 3 * kDcSlots * 8, smem + DcSmem::kRope + i * br * 128, 0, row, pg[i]);
+      }
       __syncwarp();
-      note(n + 4);
-      n += 5;
+      ++g;
       return true;
     };
     // slot order of V: value block 0 keys 0-63, 64-127, value block 1 keys 0-63, 64-127
-    auto load_v = [&](const DcSeg& s, int pages, int j) {
+    auto load_v = [&](int pages, int j) {
       int pg0[4], pg1[4];
       half_pages(pages, 0, pg0);
       half_pages(pages, 1, pg1);
-      const int sure = max(0, s.len - a.n_q + 1);  // keys that every row sees
+      const int sure = max(0, sg.len - a.n_q + 1);  // keys that every row sees
       const bool local = !E4M3 && (j + 1) * kDcTile > sure;
       if (local && one) mbar_arrive_expect_tx(fix, 4 * kDcSlotBytes);
 #pragma unroll 1
       for (int c = 0; c < 4; c += 2) {
-        if (!wait_two(n + c)) return false;
+        if (!wait_two(c)) return false;
         if (one) {
-          copy(n + c, pg0, 0, j, c + (int)rank, local);
-          copy(n + c + 1, pg1, 1, j, c + (int)rank, local);
+          copy(slot0 + c, pg0, 0, j, c + (int)rank, local);
+          copy(slot0 + c + 1, pg1, 1, j, c + (int)rank, local);
         }
         __syncwarp();
-        if (!local) { note(n + c); note(n + c + 1); }
       }
-      n += 4;
+      ++g;
       if (!local) return true;
       // some row does not see all of this tile: V came in on this CTA's own barrier; zero the rows past the
       // length, look at the rows some query may not see, then hand the slots over
@@ -459,12 +436,12 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       fix_phase ^= 1;
       uint32_t worst = 0;
       for (int c = 0; c < 4; ++c) {
-        uint8_t* base = ring + ((n - 4 + c) % kDcSlots) * kDcSlotBytes;
+        uint8_t* base = ring + (slot0 + c) * kDcSlotBytes;
         const int key0 = j * kDcTile + (c & 1) * 64;
         for (int v = max(0, sure - key0) * 16 + lane; v < 64 * 16; v += 32) {  // 16-byte pieces of rows >= sure
           const int row = v >> 4;
           uint4* p = reinterpret_cast<uint4*>(base + ((v >> 3) & 1) * 8192 + row * 128 + (v & 7) * 16);
-          if (key0 + row >= s.len) {
+          if (key0 + row >= sg.len) {
             *p = make_uint4(0u, 0u, 0u, 0u);
           } else {
             const uint4 x = *p;
@@ -483,78 +460,80 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       if (one) {
         if (rank != 0) mbar_arrive_cluster(mapa_shared(v_fixed, 0));
         else
-          for (int c = 0; c < 4; ++c) mbar_arrive(&full[(n - 4 + c) % kDcSlots]);
+          for (int c = 0; c < 4; ++c) mbar_arrive(&full[slot0 + c]);
       }
       __syncwarp();
       return true;
     };
     while (ok && it.next(a, sg)) {
       sg.uniform();
-      // the query rows of the segment before are no longer read
-      if (seg > 0 && !mbar_wait_warp(q_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
-      if (one) {
-        if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
-        tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
-      }
-      __syncwarp();
-      int pg0 = pages_of(sg, sg.k0), pg1 = pages_of(sg, sg.k0 + 1), pg2 = pages_of(sg, sg.k0 + 2);
-      ok = load_k(pg0, sg.k0);
-      if (ok && sg.k0 + 1 < sg.k1) ok = load_k(pg1, sg.k0 + 1);
-      for (int j = sg.k0; j < sg.k1 && ok; ++j) {
-        const int pg3 = pages_of(sg, j + 3);
-        ok = load_v(sg, pg0, j);
-        if (ok && j + 2 < sg.k1) ok = load_k(pg2, j + 2);
-        pg0 = pg1;
-        pg1 = pg2;
-        pg2 = pg3;
+      if (for_v) {
+        int pg = pages_of(sg.k0);
+        for (int j = sg.k0; j < sg.k1 && ok; ++j) {
+          const int next = pages_of(j + 1);
+          ok = load_v(pg, j);
+          pg = next;
+        }
+      } else {
+        // the query rows of the segment before are no longer read
+        if (seg > 0 && !mbar_wait_warp(q_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
+        if (one) {
+          if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
+          tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
+        }
+        __syncwarp();
+        int pg = pages_of(sg.k0), pg1 = pages_of(sg.k0 + 1);
+        for (int j = sg.k0; j < sg.k1 && ok; ++j) {
+          const int pg2 = pages_of(j + 2);
+          ok = load_k(pg, j);
+          pg = pg1;
+          pg1 = pg2;
+        }
       }
       ++seg;
     }
-    if (!ok && (E4M3 || rank == 0)) {  // wait (bounded) for copies in flight before the pair may leave
-      for (int s = 0; s < kDcSlots; ++s)
-        if ((issued >> s) & 1u) mbar_wait_warp(E4M3 ? &raw[s] : &full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+    if (!ok && (E4M3 || rank == 0) && g > 0) {  // wait (bounded) for the last copies before the pair may leave
+      for (int c = 0; c < 4; ++c) mbar_wait_warp(E4M3 ? &raw[slot0 + c] : &full[slot0 + c], (g - 1) & 1u, nullptr, nullptr);
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     if (rank == 0) {
       // ------------------------------------------------ MMA issuer: the warp converged, one lane issues
       constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
       constexpr uint32_t kIdescPV = idesc_f16(128, 256, ElemTraits<T>::kFmt) | kIdescBMnMajor;
       const bool one = elect_one();
-      int slot = 0, seg = 0, g = 0, n_fixed = 0;  // g: tiles of the run so far
-      uint32_t phase = 0;
+      int seg = 0, g = 0, n_fixed = 0;  // g: tiles of the run so far
       bool ok = true;
       const uint64_t dq0 = smem_desc_sw128(smem), dk0 = smem_desc_sw128(ring), dp0 = smem_desc_sw128(s_p);
-      const uint64_t dv0 = smem_desc_mn_sw128(ring, 8192);
-      auto take = [&]() {
-        ok = mbar_wait_warp(&full[slot], phase, a.status, s_abort) && ok;
+      const uint64_t dv0 = smem_desc_mn_sw128(ring + 4 * kDcSlotBytes, 8192), dr0 = smem_desc_sw128(smem + DcSmem::kRope);
+      auto wait_for = [&](uint64_t* bar, uint32_t phase) {
+        ok = mbar_wait_warp(bar, phase, a.status, s_abort) && ok;
         tc_fence_after();
       };
-      auto next_slot = [&]() {
-        if (++slot == kDcSlots) { slot = 0; phase ^= 1; }
-      };
-      auto issue_qk = [&](int tile) {
+      // S of the run's tile `tile`; last: nothing reads the segment's Q after it
+      auto issue_qk = [&](int tile, bool last) {
         const uint32_t d = tmem + kTmemS + (tile & 1) * 64;
 #pragma unroll 1
-        for (int c = 0; c < 5; ++c) {
-          take();
+        for (int c = 0; c < 4; ++c) {
+          wait_for(&full[c], tile & 1);
           if (one) {
-            const uint64_t db = dk0 + (uint32_t)slot * (kDcSlotBytes >> 4), da = dq0 + c * (16384 >> 4);
+            const uint64_t da = dq0 + c * (16384 >> 4), db = dk0 + c * (kDcSlotBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_f16_pair(d, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
-            if (c < 4) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16_pair(d, da + (8192 >> 4) + 2 * k, db + (8192 >> 4) + 2 * k, kIdescQK, 1);
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t step = (k >> 2) * (8192 >> 4) + 2 * (k & 3);
+              umma_f16_pair(d, da + step, db + step, kIdescQK, (c | k) != 0);
             }
-            umma_commit_pair_multicast(&empty[slot], 0x3);
-            if (c == 4) umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
+            umma_commit_pair_multicast(&empty[c], 0x3);
           }
           __syncwarp();
-          next_slot();
         }
-      };
-      auto free_q = [&]() {
-        if (one) umma_commit_pair_multicast(q_free, 0x3);
+        wait_for(rope_full, tile & 1);
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16_pair(d, dq0 + 8 * (8192 >> 4) + 2 * k, dr0 + 2 * k, kIdescQK, 1);
+          umma_commit_pair_multicast(rope_free, 0x3);
+          umma_commit_pair_multicast(&s_full[tile & 1], 0x3);
+          if (last) umma_commit_pair_multicast(q_free, 0x3);
+        }
         __syncwarp();
       };
       // a wait that gave up ends the loops at the next tile; until then the MMAs run on what is there
@@ -562,36 +541,30 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         sg.uniform();
         const int nt = sg.k1 - sg.k0;
         const int sure = max(0, sg.len - a.n_q + 1);
-        ok = mbar_wait_warp(q_full, seg & 1, a.status, s_abort);
-        issue_qk(g);
-        if (nt > 1) issue_qk(g + 1);
-        if (nt <= 2) free_q();
+        wait_for(q_full, seg & 1);
+        issue_qk(g, nt == 1);
+        if (nt > 1) issue_qk(g + 1, nt == 2);
         for (int j = 0; j < nt && ok; ++j) {
-          if (j == 0 && seg > 0) ok = mbar_wait_warp(o_free, (seg - 1) & 1, a.status, s_abort) && ok;
+          if (j == 0 && seg > 0) wait_for(o_free, (seg - 1) & 1);
           if (!E4M3 && (sg.k0 + j + 1) * kDcTile > sure) {
-            ok = mbar_wait_warp(v_fixed, n_fixed & 1, a.status, s_abort) && ok;
+            wait_for(v_fixed, n_fixed & 1);
             ++n_fixed;
           }
-          ok = mbar_wait_warp(p_full, (g + j) & 1, a.status, s_abort) && ok;
+          wait_for(p_full, (g + j) & 1);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            take();
+            wait_for(&full[4 + c], (g + j) & 1);
             if (one) {
-              const uint64_t db = dv0 + (uint32_t)slot * (kDcSlotBytes >> 4);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_f16_pair(tmem + (c >> 1) * 128, dp0 + (c & 1) * (8192 >> 4) + 2 * k, db + 128 * k, kIdescPV,
-                              (j | (c & 1) | k) != 0);
-              umma_commit_pair_multicast(&empty[slot], 0x3);
+                umma_f16_pair(tmem + (c >> 1) * 128, dp0 + (c & 1) * (8192 >> 4) + 2 * k,
+                              dv0 + c * (kDcSlotBytes >> 4) + 128 * k, kIdescPV, (j | (c & 1) | k) != 0);
+              umma_commit_pair_multicast(&empty[4 + c], 0x3);
               if (c == 3) umma_commit_pair_multicast(pv_done, 0x3);
             }
             __syncwarp();
-            next_slot();
           }
-          if (j + 2 < nt) {
-            issue_qk(g + j + 2);
-            if (j + 3 == nt) free_q();
-          }
+          if (j + 2 < nt) issue_qk(g + j + 2, j + 3 == nt);
         }
         g += nt;
         ++seg;
@@ -600,97 +573,91 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       __syncwarp();
       mbar_wait_warp(mma_done, 0, nullptr, nullptr);
     }
-  } else if (E4M3 && warp >= 6) {
+  } else if (E4M3 && warp >= 11) {
     // ------------------------------------------------ e4m3 codes to bf16, in place
-    // kDcTeam warps per slot and several slots at a time, so that one slot's waits lie beside the others'
-    // work. The TMA leaves the codes of key k where the second half of its bf16 row goes, so eight lanes that
-    // take a row's codes and then write both its halves need no other place, and no barrier but their warp's.
+    // kDcTeam warps to a slot, the slots of K and V in the order of their products: few warps take long over a
+    // slot, and a slot is refilled once per tile, so their time would be the tile's. The TMA leaves the codes of
+    // key k where the second half of its bf16 row goes, so eight lanes that take a row's codes and then write
+    // both its halves need no other place, and no barrier but their warp's; the scale bytes lie where other
+    // rows' first halves go, so the team takes them all before it writes.
     constexpr int kTeams = kDcConv / kDcTeam, kStride = 4 * kDcTeam;   // keys per round of a team
-    static_assert(kStride == 16, "a round is one page's keys where pages hold 16");
-    const int t = threadIdx.x - kDcThreads;
+    static_assert(4 % kTeams == 0 && 64 % kStride == 0, "teams share the slots evenly");
+    const int team = (warp - 11) / kDcTeam, t = threadIdx.x - kDcThreads;
     const int key_lo = (t >> 3) % kStride, part = t & 7;               // keys key_lo + kStride u, 16 of 128 values
-    int slot = (warp - 6) / kDcTeam;                                   // the run's slots team, team + kTeams, ...
     const uint32_t full0 = mapa_shared(full, 0);
-    DcGroups gen{it, {}, 0, 0, 0, 0, -1};
-    DcGroup grp{};
-    int c = slot;                                                      // slot of the tile's K or V
-    uint32_t phase = 0;
-    bool ok = true, more = true;
-    auto settle = [&]() {  // c counts from the group: move on to the group that holds it
-      while (more && c >= (grp.v ? 4 : 5)) {
-        c -= grp.v ? 4 : 5;
-        more = gen.next(a, grp);
-      }
-    };
-    more = gen.next(a, grp);
-    settle();
-    while (more && ok) {
-      const int half = grp.v ? (c & 1) : (int)rank, blk = grp.v ? 2 * (c >> 1) + (int)rank : c;
-      const int first = grp.j * kDcTile + half * 64;
-      uint8_t* base = ring + slot * kDcSlotBytes;
-      ok = mbar_wait_warp(&raw[slot], phase, a.status, s_abort);
-      if (blk < 4) {
-        // TMA writes start on 128 bytes: with pages of 16 keys a page's 64 scale bytes are that far apart
-        const uint8_t* sc = smem + DcSmem::kScales + slot * 512 + blk + key_lo * 4;
-        const int sc_step = a.page_size == 16 ? kStride / 16 * 128 : kStride * 4;
-        const int sure = max(0, grp.len - a.n_q + 1);
+    int seg = 0;
+    bool ok = true;
+    // this team's slots of K (for_v false) or V of key tile j, the run's tile g
+    auto widen = [&](bool for_v, int j, uint32_t g) {
+#pragma unroll 1
+      for (int c = team; c < 4; c += kTeams) {
+        const int slot = for_v ? 4 + c : c;
+        const int half = for_v ? (c & 1) : (int)rank, blk = for_v ? (c & 2) + (int)rank : c;
+        uint8_t* base = ring + slot * kDcSlotBytes;
+        const int first = j * kDcTile + half * 64;
+        ok = mbar_wait_warp(&raw[slot], g & 1u, a.status, s_abort) && ok;
+        // scale bytes: TMA writes start on 128 bytes, with pages of 16 keys a page's 64 bytes are that far apart
+        uint32_t scale[64 / kStride];
+#pragma unroll
+        for (int u = 0; u < 64 / kStride; ++u) {
+          const int key = key_lo + kStride * u;
+          scale[u] = base[blk + key * 4 + (a.page_size == 16 ? (key >> 4) * 64 : 0)];
+        }
+        ok = named_bar_and(2 + team, 32 * kDcTeam, ok);
+        const int sure = max(0, sg.len - a.n_q + 1);
         bool bad = false;
         const int sw = part >> 2, x = key_lo & 7;
         uint8_t* row = base + sw * 8192 + key_lo * 128;
         // this thread's 32 bytes of chunk part / 4: the two halves in an order that keeps eight lanes on eight banks
         const uint32_t o0 = (uint32_t)((((part & 3) * 2 + sw) ^ x) << 4), o1 = (uint32_t)((((part & 3) * 2 + 1 - sw) ^ x) << 4);
         const uint8_t* src = base + 8192 + key_lo * 128 + part * 16;
-        constexpr int kU = 2;  // keys at a time
-#pragma unroll 1
-        for (int u = 0; u < 64 / kStride; u += kU) {
-          uint32_t v0[kU][4], v1[kU][4];
-          uint2 q0[kU], q1[kU];
-          uint32_t e[kU];
 #pragma unroll
-          for (int i = 0; i < kU; ++i) {
-            q0[i] = *reinterpret_cast<const uint2*>(src + (u + i) * (kStride * 128) + 8 * sw);
-            q1[i] = *reinterpret_cast<const uint2*>(src + (u + i) * (kStride * 128) + 8 - 8 * sw);
-            e[i] = sc[(u + i) * sc_step];
-            if (first + kStride * (u + i) + key_lo >= grp.len) q0[i] = q1[i] = make_uint2(0u, 0u);
-          }
-#pragma unroll
-          for (int i = 0; i < kU; ++i) {
-            uint32_t nan = 0;
-            const uint32_t f = min(e[i] + 120u, 254u) * 0x00800080u, f2 = (e[i] - 7u) * 0x00800080u;
-            widen8(q0[i], f, e[i] > 134u, f2, nan, v0[i]);
-            widen8(q1[i], f, e[i] > 134u, f2, nan, v1[i]);
-            if (nan & 0x80808080u) {
-              nan8(q0[i], v0[i]);
-              nan8(q1[i], v1[i]);
-              bad |= first + kStride * (u + i) + key_lo >= sure;
-            }
+        for (int u = 0; u < 64 / kStride; ++u) {
+          const int key = first + kStride * u + key_lo;
+          uint2 q0 = *reinterpret_cast<const uint2*>(src + u * (kStride * 128) + 8 * sw);
+          uint2 q1 = *reinterpret_cast<const uint2*>(src + u * (kStride * 128) + 8 - 8 * sw);
+          if (key >= sg.len) q0 = q1 = make_uint2(0u, 0u);
+          uint32_t v0[4], v1[4], nan = 0;
+          const uint32_t f = min(scale[u] + 120u, 254u) * 0x00800080u, f2 = (scale[u] - 7u) * 0x00800080u;
+          widen8(q0, f, scale[u] > 134u, f2, nan, v0);
+          widen8(q1, f, scale[u] > 134u, f2, nan, v1);
+          if (nan & 0x80808080u) {
+            nan8(q0, v0);
+            nan8(q1, v1);
+            bad |= key >= sure;
           }
           __syncwarp();
-#pragma unroll
-          for (int i = 0; i < kU; ++i) {
-            *reinterpret_cast<uint4*>(row + (u + i) * (kStride * 128) + o0) = make_uint4(v0[i][0], v0[i][1], v0[i][2], v0[i][3]);
-            *reinterpret_cast<uint4*>(row + (u + i) * (kStride * 128) + o1) = make_uint4(v1[i][0], v1[i][1], v1[i][2], v1[i][3]);
-          }
+          *reinterpret_cast<uint4*>(row + u * (kStride * 128) + o0) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
+          *reinterpret_cast<uint4*>(row + u * (kStride * 128) + o1) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
         }
         // values that some query may not see must not be NaN under its P = 0
-        if (grp.v && __any_sync(0xffffffffu, bad) && lane < 2) {
-          const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (gen.seg & 1), (uint32_t)lane);
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(gen.seg + 1) : "memory");
+        if (for_v && __any_sync(0xffffffffu, bad) && lane < 2) {
+          const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
         }
         fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
-      slot += kTeams;
-      if (slot >= kDcSlots) { slot -= kDcSlots; phase ^= 1; }
-      c += kTeams;
-      settle();
+    };
+    uint32_t g = 0;  // tiles of the run before the segment
+    while (ok && it.next(a, sg)) {
+      const int nt = sg.k1 - sg.k0;
+      widen(false, sg.k0, g);
+      if (nt > 1) widen(false, sg.k0 + 1, g + 1);
+      for (int i = 0; i < nt && ok; ++i) {
+        widen(true, sg.k0 + i, g + i);
+        if (i + 2 < nt) widen(false, sg.k0 + i + 2, g + i + 2);
+      }
+      g += nt;
+      ++seg;
     }
   } else {
     // ------------------------------------------------ softmax
-    const int half = warp >> 1;                  // key half of S, value half of O
-    const int r = (warp & 1) * 32 + lane;        // row of this CTA
-    const uint32_t lane_base = tmem + ((uint32_t)warp << 21);
+    const int half = (warp >> 1) & 1, quarter = warp >> 2;  // keys 64 half + 32 quarter .. + 31 of S; values
+                                                            // 256 quarter + 128 half .. + 127 of O
+    const int r = (warp & 1) * 32 + lane;                   // row of this CTA
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);
     int seg = 0, g = 0;
     bool ok = true;
     while (ok && it.next(a, sg)) {
@@ -706,62 +673,55 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const int first = (int)(((int64_t)sg.k0 * kDcTile) >> a.page_shift);
         const int last = (int)((min((int64_t)sg.k1 * kDcTile, (int64_t)sg.len) - 1) >> a.page_shift);
         bool bad = false;
-        for (int p = first + (int)threadIdx.x; p <= last; p += 128) {
+        for (int p = first + (int)threadIdx.x; p <= last; p += kDcSoftmax) {
           const int v = __ldg(a.table + sg.b * a.ld_table + p);
           bad |= v < 0 || v >= a.num_pages;
         }
         if (bad) { record_status(a.status, MOE_ERR_INVALID_ARG); *s_badpage = seg + 1; }
-        named_bar_sync(1, 128);
+        named_bar_sync(1, kDcSoftmax);
       }
       const bool bad_page = *s_badpage == seg + 1;
       for (int j = sg.k0; j < sg.k1; ++j, ++g) {
         // a wait that gave up is carried to the next barrier of the four warps, so that all leave together
         ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
         tc_fence_after();
-        // 32 scores at a time, read twice from TMEM (maximum, then exponentials): 64 in registers beside
-        // P would not leave room for the warps that widen codes
-        const int key0 = j * kDcTile + half * 64;
+        uint32_t raw[32];
+        tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + quarter * 32, raw);
+        tmem_wait_ld();
+        const int key0 = j * kDcTile + half * 64 + quarter * 32;
         const int vis = limit - key0;
-        const bool partly = __any_sync(0xffffffffu, vis < 64);
-        auto scores = [&](int c, uint32_t (&raw)[32]) {
-          tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + c * 32, raw);
-          tmem_wait_ld();
-          if (a.neg) {
+        if (a.neg) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x) raw[x] ^= 0x80000000u;
-          }
-          if (partly) {
+          for (int x = 0; x < 32; ++x) raw[x] ^= 0x80000000u;
+        }
+        if (__any_sync(0xffffffffu, vis < 32)) {
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (c * 32 + x >= vis) raw[x] = 0xFF800000u;
-          }
-          if (bad_page) {
+          for (int x = 0; x < 32; ++x)
+            if (x >= vis) raw[x] = 0xFF800000u;
+        }
+        if (bad_page) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int64_t pi = ((int64_t)key0 + c * 32 + u * 16) >> a.page_shift;
-              const int v = pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
-              if (v < 0 || v >= a.num_pages) {
+          for (int u = 0; u < 2; ++u) {
+            const int64_t pi = ((int64_t)key0 + u * 16) >> a.page_shift;
+            const int v = pi < a.table_width ? __ldg(a.table + sg.b * a.ld_table + pi) : -1;
+            if (v < 0 || v >= a.num_pages) {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) raw[u * 16 + x] = 0xFF800000u;
-              }
+              for (int x = 0; x < 16; ++x) raw[u * 16 + x] = 0xFF800000u;
             }
           }
-        };
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          uint32_t raw[32];
-          scores(c, raw);
-#pragma unroll
-          for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[x]));
         }
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // the row's other 64 keys are with the thread 64 further on
-        float* x = s_x + (g & 1) * 128;
-        x[threadIdx.x] = top;
-        ok = named_bar_and(1, 128, ok);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[x]));
+        // the row's other keys are with three other threads. Any common reference near the maximum will do:
+        // they exchange it rounded up to bf16, two tiles' worth in turn
+        __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(s_x) + (g & 1) * kDcSoftmax;
+        x[threadIdx.x] = __float2bfloat16_ru(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        ok = named_bar_and(1, kDcSoftmax, ok);
         if (!ok) break;
-        top = fmaxf(top, x[threadIdx.x ^ 64]) * a.scale_log2;
+        const float top = fmaxf(fmaxf(__bfloat162float(x[threadIdx.x]), __bfloat162float(x[threadIdx.x ^ 64])),
+                                fmaxf(__bfloat162float(x[threadIdx.x ^ 128]), __bfloat162float(x[threadIdx.x ^ 192]))) *
+                          a.scale_log2;
         const bool move = top > m_ref + kDcRescaleLog2 || m_ref == -INFINITY;
         float f = 1.0f;
         if (move) {
@@ -771,19 +731,14 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         const float base = m_ref == -INFINITY ? 0.f : m_ref;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t p[32];
+        uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t raw[32];
-          scores(c, raw);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = ex2d(fmaf(__uint_as_float(raw[2 * e]), a.scale_log2, -base));
-            const float p1 = ex2d(fmaf(__uint_as_float(raw[2 * e + 1]), a.scale_log2, -base));
-            sum[e & 1] += p0;
-            sum[2 + (e & 1)] += p1;
-            p[c * 16 + e] = ElemTraits<T>::pack2(p0, p1);
-          }
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = ex2d(fmaf(__uint_as_float(raw[2 * e]), a.scale_log2, -base));
+          const float p1 = ex2d(fmaf(__uint_as_float(raw[2 * e + 1]), a.scale_log2, -base));
+          sum[e & 1] += p0;
+          sum[2 + (e & 1)] += p1;
+          p[e] = ElemTraits<T>::pack2(p0, p1);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (j > sg.k0) {  // PV of the tile before: its P is read, its O is written
@@ -792,21 +747,21 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (__any_sync(0xffffffffu, move && f != 1.0f)) {
             const float w = move ? f : 1.0f;
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < 4; ++c) {
               uint32_t o[32];
-              tmem_ld32(lane_base + c * 32, o);
+              tmem_ld32(lane_base + quarter * 128 + c * 32, o);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w);
-              tmem_st32(lane_base + c * 32, o);
+              tmem_st32(lane_base + quarter * 128 + c * 32, o);
             }
             tmem_wait_st();
           }
         }
         uint8_t* dst = s_p + half * 8192 + r * 128;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(dst + ((c ^ (r & 7)) << 4)) =
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint4*>(dst + (((quarter * 4 + c) ^ (r & 7)) << 4)) =
               make_uint4(p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
         fence_proxy_async_smem();
         tc_fence_before();
@@ -816,11 +771,12 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       ok = ok && mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort);
       tc_fence_after();
       // ---------------------------------------------- end of the segment
-      ok = named_bar_and(1, 128, ok);  // the maxima of the last tile are read
+      ok = named_bar_and(1, kDcSoftmax, ok);  // the maxima of the last tile are read
       if (!ok) break;
       s_x[threadIdx.x] = l;
-      named_bar_sync(1, 128);
-      l += s_x[threadIdx.x ^ 64];
+      named_bar_sync(1, kDcSoftmax);
+      // in one order for all four: the same sum
+      l = (s_x[r] + s_x[r + 64]) + (s_x[r + 128] + s_x[r + 192]);
       const bool whole = sg.k0 == 0 && sg.k1 == sg.n;
       const int64_t pslot = 2 * pair + (sg.k0 == 0 ? 1 : 0);
       const bool live = row < a.rows;
@@ -828,7 +784,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(o_free, 0));
-        for (int rr = warp; rr < kDcRows; rr += 4) {
+        for (int rr = warp; rr < kDcRows; rr += kDcSoftmax / 32) {
           const int rw = sg.rt * kDcTile + (int)rank * kDcRows + rr;
           if (rw >= a.rows) break;
           float m, ls, acc[16];
@@ -854,11 +810,11 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const bool some = l > 0.f || l != l;
         const float inv = some ? 1.0f / l : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {  // TMEM columns 32 c: values 256 (c / 4) + 128 half + 32 (c % 4)
+        for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          tmem_ld32(lane_base + c * 32, o);
+          tmem_ld32(lane_base + quarter * 128 + c * 32, o);
           tmem_wait_ld();
-          const int d = (c >> 2) * 256 + half * 128 + (c & 3) * 32;
+          const int d = quarter * 256 + half * 128 + c * 32;
           if (live) {
             if (whole) {
               uint4* dst =
@@ -880,7 +836,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             }
           }
         }
-        if (live && half == 0) {
+        if (live && half == 0 && quarter == 0) {
           if (!whole) a.part_ml[pslot * a.part_rows + (int)rank * kDcRows + r] = make_float2(m_ref, l);
           else if (a.lse != nullptr)
             a.lse[(int64_t)sg.b * a.rows + row] = some ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
@@ -889,7 +845,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(o_free, 0));
       }
-      named_bar_sync(1, 128);  // s_x is free again
+      named_bar_sync(1, kDcSoftmax);  // s_x is free again
       ++seg;
     }
   }
@@ -898,7 +854,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while its peer may use its barriers, shared memory or TMEM
   tc_fence_after();
-  if (warp == 5) tmem_dealloc_pair(tmem, 512);
+  if (warp == 9) tmem_dealloc_pair(tmem, 512);
 }
 
 // Joins the pieces of requests that several pairs worked on, and writes the rows of empty ones: one
@@ -1012,8 +968,10 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   } else {
     const uint64_t dc[4] = {64, (uint64_t)a.page_size, kRowDim / 64, (uint64_t)a.num_pages};
     const uint64_t sc[3] = {row, 128, row * (uint64_t)a.page_size};
-    maps = maps && make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1);
-    mr = ms = mc;
+    const uint64_t dr[3] = {kRopeDim, (uint64_t)a.page_size, (uint64_t)a.num_pages}, sr[2] = {row, sc[2]};
+    maps = maps && make_chunks_map(&mc, dtype, a.cache, dc, sc, box_rows, box_rows == 64 ? 2 : 1) &&
+           make_kmajor_map(&mr, dtype, a.cache + 2 * kLatDim, 3, dr, sr, box_rows);
+    ms = mc;
   }
   if (!maps) return cudaErrorInvalidValue;
   auto kern = latent_decode_kernel<T, E4M3>;
