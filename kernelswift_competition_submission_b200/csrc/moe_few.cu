@@ -13,21 +13,31 @@
 //
 // The k order inside an MMA is free as long as both operands agree, so a lane takes 32
 // consecutive bytes of its row per 128-byte block (four lanes read one full line) and feeds
-// them to 8 (e4m3) or 4 (16-bit) MMAs in the order they lie. e4m3 codes become 16-bit floats
-// by moving their bits: the code's exponent and fraction land in the low end of the wider
-// exponent field, which is the value times 2^-120 (bf16) or 2^-8 (fp16) exactly, subnormals
-// included; the power goes back exactly in a bf16 multiply, or for fp16 in the block scale.
+// them to 8 (e4m3) or 4 (16-bit) MMAs in the order they lie. e4m3 codes become fp16 pairs with
+// the conversion instruction (moving their bits to bf16 by shifts and masks instead kept the
+// integer pipe busier than HBM: 0.53 against 0.58 of its rate in few_up at one token, 0.53 against
+// 0.64 in few_down at eight), so bf16 tokens and bf16 a_p rows become fp16 too, each row under
+// the power of two that brings its largest magnitude to 2^14 .. 2^15: what lies below 2^-39 of
+// that maximum is lost, far under the bf16 rounding of the same row.
 //
-// few_up:   one warp per item (chunk of up to 8 pairs of one expert, 8 columns of N): rows 0-7
-//           of the A operand are gate rows, rows 8-15 the same up rows, so a lane holds both
-//           halves of its SiLU * mul. Every CTA routes all tokens itself (a warp per token).
-// few_down: one CTA per 16 rows of the output; its warps take consecutive runs of the
-//           (chunk, k block) list, add weight * product into their own shared rows in fp32,
-//           and the rows are summed in warp order: the same bits on every run.
-// Sums are fp32; a_p is rounded once to the tokens' type (the layer's other paths do the same).
+// few_up:   items of 8 columns of N for a chunk of up to 8 pairs of one expert: rows 0-7 of the A
+//           operand are gate rows, rows 8-15 the same up rows, so a lane holds both halves of its
+//           SiLU * mul. Every CTA routes all tokens itself (a warp per token), takes an equal run
+//           of the items and gives each of its 16 warps an equal run of their k blocks, whatever
+//           the number of items; items cut between warps are joined in shared memory in order.
+// few_down: one CTA per 16 rows of the output; its warps take consecutive runs of the (chunk, k
+//           block) list, add weight * product into their own shared rows in fp32, and the rows are
+//           summed in warp order. It is launched while few_up still runs and waits for it on the
+//           device.
+// Both give the same bits on every run. Sums are fp32; a_p is rounded once to the tokens' type (the
+// layer's other paths do the same).
 #include "common.cuh"
 #include "moe_internal.h"
 #include "routing.cuh"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
 
 namespace moe {
 namespace {
@@ -36,7 +46,7 @@ constexpr int kFewMaxTokens = 32;
 constexpr int kFewMaxPairs = 512;
 constexpr int kFewCols = 8;          // pairs per chunk: the MMA's columns
 constexpr int kUpWarps = 16;
-constexpr int kDownWarps = 8;
+constexpr int kDownMaxWarps = 16;
 constexpr int kBlkBytes = 128;       // weight bytes of a row per k block
 
 // Written by few_up's first CTA for few_down.
@@ -46,6 +56,7 @@ struct FewTables {
   int32_t chunk_expert[kFewMaxPairs];
   int16_t chunk_pair[kFewMaxPairs][kFewCols];      // pair t * topk + slot, -1 for an empty column
   float weight[kFewMaxPairs];                      // by pair
+  uint32_t amax[kFewMaxPairs];                     // by pair: largest |a| as float bits (e4m3 weights, bf16 tokens)
 };
 
 struct FewRouting {
@@ -53,6 +64,7 @@ struct FewRouting {
   const float* bias;
   int topk, renormalize, n_group, topk_group, scoring, gmode;
   float scale;
+  bool aligned;  // logits and bias on 16 bytes
 };
 
 __device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
@@ -85,86 +97,90 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], uint32_t a0, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Four e4m3 codes -> (codes 0, 2) and (codes 1, 3) as pairs of T. The bit move would turn e4m3
-// NaN into 480, so block_mma notes NaN codes per row and the row's results become NaN.
-template <typename T> struct Expand8;
-template <> struct Expand8<__nv_bfloat16> {
-  static constexpr float kScale = 1.0f;
-  __device__ static __forceinline__ uint32_t lift(uint32_t w) {  // codes in the high byte of each half
-    const uint32_t b = (w & 0x80008000u) | ((w >> 4) & 0x07F007F0u);
-    uint32_t r;  // * 2^120
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(b), "r"(0x7B807B80u));
-    return r;
-  }
-};
-template <> struct Expand8<__half> {
-  static constexpr float kScale = 256.0f;  // joins the block scale
-  __device__ static __forceinline__ uint32_t lift(uint32_t w) { return (w & 0x80008000u) | ((w >> 1) & 0x3F803F80u); }
-};
+// Two e4m3 codes (the low half of w) as an fp16 pair; NaN codes stay NaN.
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The power of two that brings a largest magnitude (as float bits) into [2^14, 2^15); 1 for a row of
+// zeros and for one that holds infinities or NaN.
+__device__ __forceinline__ float row_scale(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23);
+  return e == 0 || e == 255 ? 1.0f : __int_as_float(min(max(127 + 14 - (e - 127), 1), 254) << 23);
+}
 
-// The tokens' side of one k block: 32 or 16 consecutive values of this lane's column.
-template <int WORDS>
-__device__ __forceinline__ void load_col(const uint8_t* p, uint32_t (&x)[WORDS]) {
+// The tokens' side of one k block: 32 or 16 consecutive values of this lane's column, zeros without one.
+// With e4m3 weights the values are wanted in fp16: bf16 ones are scaled and converted.
+template <typename T, bool F8>
+__device__ __forceinline__ void load_col(const T* p, float scale, uint32_t (&x)[F8 ? 16 : 8]) {
 #pragma unroll
-  for (int i = 0; i < WORDS / 4; ++i) {
-    const uint4 v = p ? *reinterpret_cast<const uint4*>(p + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < (F8 ? 4 : 2); ++i) {
+    uint4 v = p ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
     x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+  }
+  if constexpr (F8 && ElemTraits<T>::kFmt == 1) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float lo = __uint_as_float(x[i] << 16) * scale, hi = __uint_as_float(x[i] & 0xFFFF0000u) * scale;
+      x[i] = ElemTraits<__half>::pack2(lo, hi);
+    }
   }
 }
 
 // One 128-byte k block: rows lo (A rows 0-7) and hi (A rows 8-15), 32 bytes each per lane.
 template <typename T, bool F8>
 __device__ __forceinline__ void block_mma(float (&c)[4], const uint4 (&lo)[2], const uint4 (&hi)[2],
-                                          const uint32_t (&x)[F8 ? 16 : 8], uint32_t& nan_lo, uint32_t& nan_hi) {
+                                          const uint32_t (&x)[F8 ? 16 : 8]) {
   const uint32_t l[8] = {lo[0].x, lo[0].y, lo[0].z, lo[0].w, lo[1].x, lo[1].y, lo[1].z, lo[1].w};
   const uint32_t h[8] = {hi[0].x, hi[0].y, hi[0].z, hi[0].w, hi[1].x, hi[1].y, hi[1].z, hi[1].w};
   if constexpr (F8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      nan_lo |= (l[i] & 0x7F7F7F7Fu) + 0x01010101u;  // bit 7 of a byte: the code was NaN
-      nan_hi |= (h[i] & 0x7F7F7F7Fu) + 0x01010101u;
-      const uint32_t b0 = __byte_perm(x[2 * i], x[2 * i + 1], 0x5410);  // values 0, 2 of the four
-      const uint32_t b1 = __byte_perm(x[2 * i], x[2 * i + 1], 0x7632);  // values 1, 3
-      mma16816<T>(c, Expand8<T>::lift(l[i] << 8), Expand8<T>::lift(h[i] << 8), Expand8<T>::lift(l[i]),
-                  Expand8<T>::lift(h[i]), b0, b1);
-    }
+    for (int i = 0; i < 8; ++i)
+      mma16816<__half>(c, widen2(l[i] & 0xFFFFu), widen2(h[i] & 0xFFFFu), widen2(l[i] >> 16), widen2(h[i] >> 16),
+                       x[2 * i], x[2 * i + 1]);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) mma16816<T>(c, l[2 * i], h[2 * i], l[2 * i + 1], h[2 * i + 1], x[2 * i], x[2 * i + 1]);
   }
 }
 
-// The quad's four lanes hold one row's k values: a NaN code in any of them makes the row NaN.
-__device__ __forceinline__ void poison_rows(float (&acc)[4], uint32_t nan_lo, uint32_t nan_hi) {
-  uint32_t f = ((nan_lo & 0x80808080u) ? 1u : 0u) | ((nan_hi & 0x80808080u) ? 2u : 0u);
-  f |= __shfl_xor_sync(0xffffffffu, f, 1);
-  f |= __shfl_xor_sync(0xffffffffu, f, 2);
-  if (f & 1u) acc[0] = acc[1] = __int_as_float(0x7FC00000);
-  if (f & 2u) acc[2] = acc[3] = __int_as_float(0x7FC00000);
-}
-
+// The routing of one token by one warp, as moe_grouped_topk does it.
 __device__ __forceinline__ void route_one(const FewRouting& r, int tok, int E, float* w, int32_t* ids,
-                                          float* s_choice) {
+                                          float* s_choice, RouteScratch* scr) {
   const float* row = r.logits + (int64_t)tok * E;
-  if (E <= 64)
+  const bool grouped = r.topk_group < r.n_group;
+  // 256 experts, without groups or in groups of 64 or 32: the register-only rule (1 us less per token)
+  if (E == 256 && r.aligned && (!grouped || r.n_group == 4 || r.n_group == 8)) {
+#define MOE_ROUTE(LPG)                                                                                             \
+  route_token_lanes<8, LPG, false>(row, r.bias, tok, r.topk, r.renormalize, r.n_group, r.topk_group, r.scoring, r.gmode, \
+                                   r.scale, w, ids, scr)
+    if (grouped && r.n_group == 8) MOE_ROUTE(4);
+    else if (grouped) MOE_ROUTE(8);
+    else MOE_ROUTE(1);
+#undef MOE_ROUTE
+  } else if (E <= 64) {
     route_token_general<2, false>(row, r.bias, tok, E, r.topk, r.renormalize, r.n_group, r.topk_group, r.scoring,
                                   r.gmode, r.scale, w, ids, s_choice);
-  else if (E <= 256)
+  } else if (E <= 256) {
     route_token_general<8, false>(row, r.bias, tok, E, r.topk, r.renormalize, r.n_group, r.topk_group, r.scoring,
                                   r.gmode, r.scale, w, ids, s_choice);
-  else
+  } else {
     route_token_general<16, false>(row, r.bias, tok, E, r.topk, r.renormalize, r.n_group, r.topk_group, r.scoring,
                                    r.gmode, r.scale, w, ids, s_choice);
+  }
 }
 
 struct UpShared {
+  RouteScratch scratch[kUpWarps];
   float choice[kUpWarps][kRouteMaxExperts];
   float weight[kFewMaxPairs];
   int32_t id[kFewMaxPairs];
   int32_t count[kRouteMaxExperts];   // pairs of an expert, then its first chunk
   int32_t chunk_expert[kFewMaxPairs];
   int16_t chunk_pair[kFewMaxPairs][kFewCols];
+  float scale[kFewMaxTokens];        // by token, e4m3 weights and bf16 tokens
   int32_t n_chunks;
+  alignas(16) float part[kUpWarps][2][32][4];  // a warp's sums of an item that it did not begin / did not end
 };
 
 template <typename T, bool F8>
@@ -173,11 +189,24 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
               const float* __restrict__ w1s, int M, int E, int K, int N, T* __restrict__ act, FewTables* tab) {
   extern __shared__ __align__(16) uint8_t smem_up[];
   UpShared& s = *reinterpret_cast<UpShared*>(smem_up);
+  constexpr bool kToHalf = F8 && ElemTraits<T>::kFmt == 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int P = M * rt.topk;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int t = warp; t < M; t += kUpWarps) {
-    route_one(rt, t, E, s.weight, s.id, s.choice[warp]);
+    route_one(rt, t, E, s.weight, s.id, s.choice[warp], &s.scratch[warp]);
     __syncwarp();
+    if constexpr (kToHalf) {
+      uint32_t m = 0;
+      for (int i = lane * 8; i < K; i += 256) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)t * ld_x + i);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max(w[j] << 16 & 0x7FFF0000u, w[j] & 0x7FFF0000u));
+      }
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (lane == 0) s.scale[t] = row_scale(m);
+    }
   }
   for (int i = threadIdx.x; i < E; i += blockDim.x) s.count[i] = 0;
   for (int i = threadIdx.x; i < kFewMaxPairs * kFewCols / 2; i += blockDim.x)
@@ -230,91 +259,147 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
 
   constexpr int kElt = F8 ? 1 : 2;                // weight bytes per element
   constexpr int kBlkElts = kBlkBytes / kElt;      // elements of a k block
-  constexpr int kWords = F8 ? 16 : 8;             // 32-bit words of x per lane and block
+  constexpr int kColElts = kBlkElts / 4;          // of them per lane
   constexpr int kDepth = 3;                       // k blocks in flight per lane
   const int g = lane >> 2, t4 = lane & 3;
   const int nkb = K / kBlkElts;
   const int NB = N / 8;
-  const int items = s.n_chunks * NB;
+  const int64_t items = (int64_t)s.n_chunks * NB;
   const int64_t row_bytes = (int64_t)K * kElt;
-  for (int it = blockIdx.x * kUpWarps + warp; it < items; it += gridDim.x * kUpWarps) {
-    const int c = it / NB, n0 = (it - c * NB) * 8;
-    const int e = s.chunk_expert[c];
-    const uint8_t* lo_p = w1 + ((int64_t)e * 2 * N + n0 + g) * row_bytes + t4 * 32;
-    const uint8_t* hi_p = lo_p + (int64_t)N * row_bytes;
+  const int64_t i0 = items * blockIdx.x / gridDim.x, i1 = items * (blockIdx.x + 1) / gridDim.x;
+  const int blocks = (int)(i1 - i0) * nkb;
+  auto begin_of = [&](int w) { return (int)((int64_t)blocks * w / kUpWarps); };
+  const int b0 = begin_of(warp), b1 = begin_of(warp + 1);
+
+  // item `it` (of this CTA): its gate row for this lane; the up row is N rows further on
+  auto row_of = [&](int it) {
+    const int64_t i = i0 + it;
+    const int c = (int)(i / NB), n0 = (int)(i - (int64_t)c * NB) * 8;
+    return w1 + ((int64_t)s.chunk_expert[c] * 2 * N + n0 + g) * row_bytes + t4 * 32;
+  };
+  const int64_t up = (int64_t)N * row_bytes;
+  int l_it = b0 / nkb, l_k = b0 - l_it * nkb, left = b1 - b0;  // the next block to load
+  const uint8_t* lp = left > 0 ? row_of(l_it) : nullptr;
+  uint4 lo[kDepth][2], hi[kDepth][2];
+  auto load = [&](int d) {
+    const uint8_t* p = lp + (int64_t)l_k * kBlkBytes;
+    lo[d][0] = ldg_stream(p);
+    lo[d][1] = ldg_stream(p + 16);
+    hi[d][0] = ldg_stream(p + up);
+    hi[d][1] = ldg_stream(p + up + 16);
+    --left;
+    if (++l_k == nkb) {
+      l_k = 0;
+      ++l_it;
+      if (left > 0) lp = row_of(l_it);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d)
+    if (left > 0) load(d);
+
+  int it = b0 / nkb, kb = b0 - it * nkb;
+  bool begun = kb == 0;  // this warp has the item from its first block on
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const T* xp = nullptr;
+  float xs = 1.0f;
+  const float* sg = nullptr;
+  const float* su = nullptr;
+  auto open_item = [&]() {
+    const int64_t i = i0 + it;
+    const int c = (int)(i / NB), n0 = (int)(i - (int64_t)c * NB) * 8;
     const int pair = s.chunk_pair[c][g];
-    const uint8_t* xp = pair >= 0
-                            ? reinterpret_cast<const uint8_t*>(x + (int64_t)(pair / rt.topk) * ld_x) + t4 * (kWords * 4)
-                            : nullptr;
-    const float* sg = nullptr;
-    const float* su = nullptr;
+    xp = pair >= 0 ? x + (int64_t)(pair / rt.topk) * ld_x + t4 * kColElts : nullptr;
+    if constexpr (kToHalf) xs = pair >= 0 ? s.scale[pair / rt.topk] : 1.0f;
     if constexpr (F8) {
-      sg = w1s + ((int64_t)e * (2 * N / 128) + n0 / 128) * (K / 128);
+      sg = w1s + ((int64_t)s.chunk_expert[c] * (2 * N / 128) + n0 / 128) * (K / 128);
       su = sg + (int64_t)(N / 128) * (K / 128);
     }
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t nan_lo = 0, nan_hi = 0;
-    uint4 lo[kDepth][2], hi[kDepth][2];
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      if (d < nkb) {
-        lo[d][0] = ldg_stream(lo_p + d * kBlkBytes);
-        lo[d][1] = ldg_stream(lo_p + d * kBlkBytes + 16);
-        hi[d][0] = ldg_stream(hi_p + d * kBlkBytes);
-        hi[d][1] = ldg_stream(hi_p + d * kBlkBytes + 16);
-      }
-    }
-    for (int kb0 = 0; kb0 < nkb; kb0 += kDepth) {
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int kb = kb0 + d;
-        if (kb < nkb) {
-          uint32_t xv[kWords];
-          load_col<kWords>(xp ? xp + (int64_t)kb * (kBlkElts * 2) : nullptr, xv);
-          if constexpr (F8) {
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
-            block_mma<T, F8>(part, lo[d], hi[d], xv, nan_lo, nan_hi);
-            const float a = __ldg(sg + kb) * Expand8<T>::kScale, b = __ldg(su + kb) * Expand8<T>::kScale;
-            acc[0] = fmaf(a, part[0], acc[0]);
-            acc[1] = fmaf(a, part[1], acc[1]);
-            acc[2] = fmaf(b, part[2], acc[2]);
-            acc[3] = fmaf(b, part[3], acc[3]);
-          } else {
-            block_mma<T, F8>(acc, lo[d], hi[d], xv, nan_lo, nan_hi);
-          }
-          const int nx = kb + kDepth;
-          if (nx < nkb) {
-            lo[d][0] = ldg_stream(lo_p + (int64_t)nx * kBlkBytes);
-            lo[d][1] = ldg_stream(lo_p + (int64_t)nx * kBlkBytes + 16);
-            hi[d][0] = ldg_stream(hi_p + (int64_t)nx * kBlkBytes);
-            hi[d][1] = ldg_stream(hi_p + (int64_t)nx * kBlkBytes + 16);
-          }
-        }
-      }
-    }
-    if constexpr (F8) poison_rows(acc, nan_lo, nan_hi);
-    // this lane: row n0 + g of gate (acc 0, 1) and up (acc 2, 3) for columns 2 t4, 2 t4 + 1
+  };
+  // this lane: row n0 + g of gate (a 0, 1) and up (a 2, 3) for columns 2 t4, 2 t4 + 1
+  auto finish = [&](int item, const float (&a)[4]) {
+    const int64_t i = i0 + item;
+    const int c = (int)(i / NB), n0 = (int)(i - (int64_t)c * NB) * 8;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int pj = s.chunk_pair[c][2 * t4 + j];
+      float v = 0.f;
       if (pj >= 0) {
-        const float gate = acc[j], up = acc[2 + j];
-        act[(int64_t)pj * N + n0 + g] = ElemTraits<T>::from_float(gate / (1.0f + expf(-gate)) * up);
+        const float r = kToHalf ? 1.0f / s.scale[pj / rt.topk] : 1.0f;  // a power of two
+        const float gate = a[j] * r, upv = a[2 + j] * r;
+        const T q = ElemTraits<T>::from_float(gate / (1.0f + expf(-gate)) * upv);
+        act[(int64_t)pj * N + n0 + g] = q;
+        v = fabsf((float)q);
+      }
+      if constexpr (kToHalf) {
+        // the pair's largest magnitude over the item's 8 rows, then over all items; a maximum needs no order
+        uint32_t m = __float_as_uint(v);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (g == 0 && pj >= 0) atomicMax(&tab->amax[pj], m);
       }
     }
+  };
+  if (b0 < b1) open_item();
+  for (int b = b0; b < b1; b += kDepth) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      if (b + d < b1) {
+        uint32_t xv[F8 ? 16 : 8];
+        load_col<T, F8>(xp ? xp + (int64_t)kb * kBlkElts : nullptr, xs, xv);
+        if constexpr (F8) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          block_mma<T, F8>(part, lo[d], hi[d], xv);
+          const float a = __ldg(sg + kb), u = __ldg(su + kb);
+          acc[0] = fmaf(a, part[0], acc[0]);
+          acc[1] = fmaf(a, part[1], acc[1]);
+          acc[2] = fmaf(u, part[2], acc[2]);
+          acc[3] = fmaf(u, part[3], acc[3]);
+        } else {
+          block_mma<T, F8>(acc, lo[d], hi[d], xv);
+        }
+        if (left > 0) load(d);
+        if (++kb == nkb) {
+          if (begun) finish(it, acc);
+          else *reinterpret_cast<float4*>(s.part[warp][0][lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = 0.f;
+          kb = 0;
+          ++it;
+          begun = true;
+          if (b + d + 1 < b1) open_item();
+        }
+      }
+    }
+  }
+  if (b0 < b1 && kb != 0)
+    *reinterpret_cast<float4*>(s.part[warp][begun ? 1 : 0][lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (b0 < b1 && kb != 0 && begun) {  // this warp began the item: it adds what the next ones have of it
+    const int end = (it + 1) * nkb;
+    for (int w = warp + 1; w < kUpWarps && begin_of(w) < end; ++w) {
+      if (begin_of(w) == begin_of(w + 1)) continue;
+      const float4 v = *reinterpret_cast<const float4*>(s.part[w][0][lane]);
+      acc[0] += v.x;
+      acc[1] += v.y;
+      acc[2] += v.z;
+      acc[3] += v.w;
+    }
+    finish(it, acc);
   }
 }
 
 template <typename T, bool F8>
-__global__ void __launch_bounds__(32 * kDownWarps)
+__global__ void __launch_bounds__(32 * kDownMaxWarps)
 few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, const uint8_t* __restrict__ w2,
                 const float* __restrict__ w2s, int M, int topk, int K, int N, T* __restrict__ out) {
-  extern __shared__ __align__(16) float s_part[];  // [kDownWarps][M][16]
+  extern __shared__ __align__(16) float s_part[];  // [warps][M][16]
+  constexpr bool kToHalf = F8 && ElemTraits<T>::kFmt == 1;
   constexpr int kElt = F8 ? 1 : 2;
   constexpr int kBlkElts = kBlkBytes / kElt;
-  constexpr int kWords = F8 ? 16 : 8;
+  constexpr int kColElts = kBlkElts / 4;
   constexpr int kDepth = 3;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const int h0 = blockIdx.x * 16;
   const int nkb = N / kBlkElts;
@@ -322,13 +407,13 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
   float* mine = s_part + warp * M * 16;
   for (int i = lane; i < M * 16; i += 32) mine[i] = 0.f;
   __syncwarp();
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // few_up's rows and tables
   const int total = tab->n_chunks * nkb;
-  const int b0 = (int)((int64_t)total * warp / kDownWarps), b1 = (int)((int64_t)total * (warp + 1) / kDownWarps);
+  const int b0 = (int)((int64_t)total * warp / warps), b1 = (int)((int64_t)total * (warp + 1) / warps);
 
-  int lc = b0 / nkb, lk = b0 - lc * nkb;  // the next block to load
-  const uint8_t* lp = nullptr;
-  auto row_of = [&](int c) { return w2 + ((int64_t)__ldg(&tab->chunk_expert[c]) * K + h0 + g) * row_bytes + t4 * 32; };
-  if (b0 < b1) lp = row_of(lc);
+  int lc = b0 / nkb, lk = b0 - lc * nkb, left = b1 - b0;  // the next block to load
+  auto row_of = [&](int c) { return w2 + ((int64_t)tab->chunk_expert[c] * K + h0 + g) * row_bytes + t4 * 32; };
+  const uint8_t* lp = left > 0 ? row_of(lc) : nullptr;
   uint4 lo[kDepth][2], hi[kDepth][2];
   auto load = [&](int d) {
     const uint8_t* p = lp + (int64_t)lk * kBlkBytes;
@@ -336,9 +421,6 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
     lo[d][1] = ldg_stream(p + 16);
     hi[d][0] = ldg_stream(p + 8 * row_bytes);
     hi[d][1] = ldg_stream(p + 8 * row_bytes + 16);
-  };
-  int left = b1 - b0;  // blocks not yet loaded
-  auto advance = [&]() {
     --left;
     if (++lk == nkb) {
       lk = 0;
@@ -348,31 +430,29 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
   };
 #pragma unroll
   for (int d = 0; d < kDepth; ++d)
-    if (left > 0) { load(d); advance(); }
+    if (left > 0) load(d);
 
   int c = b0 < b1 ? b0 / nkb : 0, kb = b0 < b1 ? b0 - c * nkb : 0;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  uint32_t nan_lo = 0, nan_hi = 0;
-  const uint8_t* xp = nullptr;
+  const T* xp = nullptr;
+  float xs = 1.0f;
   const float* sp = nullptr;
   auto open_chunk = [&]() {
     const int pair = tab->chunk_pair[c][g];
-    xp = pair >= 0 ? reinterpret_cast<const uint8_t*>(act + (int64_t)pair * N) + t4 * (kWords * 4) : nullptr;
+    xp = pair >= 0 ? act + (int64_t)pair * N + t4 * kColElts : nullptr;
+    if constexpr (kToHalf) xs = pair >= 0 ? row_scale(tab->amax[pair]) : 1.0f;
     if constexpr (F8) sp = w2s + ((int64_t)tab->chunk_expert[c] * (K / 128) + h0 / 128) * (N / 128);
   };
   auto close_chunk = [&]() {
-    if constexpr (F8) {
-      poison_rows(acc, nan_lo, nan_hi);
-      nan_lo = nan_hi = 0;
-    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int p = tab->chunk_pair[c][2 * t4 + j];
       if (p >= 0) {
+        const float r = kToHalf ? 1.0f / row_scale(tab->amax[p]) : 1.0f;  // a power of two
         const float w = tab->weight[p];
         float* o = mine + (p / topk) * 16 + g;
-        o[0] += w * acc[j];
-        o[8] += w * acc[2 + j];
+        o[0] += w * (acc[j] * r);
+        o[8] += w * (acc[2 + j] * r);
       }
     }
     __syncwarp();
@@ -384,18 +464,18 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       if (b + d < b1) {
-        uint32_t xv[kWords];
-        load_col<kWords>(xp ? xp + (int64_t)kb * (kBlkElts * 2) : nullptr, xv);
+        uint32_t xv[F8 ? 16 : 8];
+        load_col<T, F8>(xp ? xp + (int64_t)kb * kBlkElts : nullptr, xs, xv);
         if constexpr (F8) {
           float part[4] = {0.f, 0.f, 0.f, 0.f};
-          block_mma<T, F8>(part, lo[d], hi[d], xv, nan_lo, nan_hi);
-          const float a = __ldg(sp + kb) * Expand8<T>::kScale;
+          block_mma<T, F8>(part, lo[d], hi[d], xv);
+          const float a = __ldg(sp + kb);
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j] = fmaf(a, part[j], acc[j]);
         } else {
-          block_mma<T, F8>(acc, lo[d], hi[d], xv, nan_lo, nan_hi);
+          block_mma<T, F8>(acc, lo[d], hi[d], xv);
         }
-        if (left > 0) { load(d); advance(); }
+        if (left > 0) load(d);
         if (++kb == nkb) {
           close_chunk();
           kb = 0;
@@ -409,8 +489,7 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
   __syncthreads();
   for (int i = threadIdx.x; i < M * 16; i += blockDim.x) {
     float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDownWarps; ++w) v += s_part[w * M * 16 + i];
+    for (int w = 0; w < warps; ++w) v += s_part[w * M * 16 + i];
     const int t = i >> 4;
     if (tab->bad[t]) v = __int_as_float(0x7FC00000);
     out[(int64_t)t * K + h0 + (i & 15)] = ElemTraits<T>::from_float(v);
@@ -428,12 +507,28 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
   T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(ws) + few_tables_bytes());
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(few_up_kernel<T, F8>), (int)sizeof(UpShared));
   if (err != cudaSuccess) return err;
+  if (F8 && ElemTraits<T>::kFmt == 1) {
+    err = cudaMemsetAsync(tab->amax, 0, sizeof(uint32_t) * (size_t)M * rt.topk, st);
+    if (err != cudaSuccess) return err;
+  }
   few_up_kernel<T, F8><<<num_sms(), 32 * kUpWarps, sizeof(UpShared), st>>>(
       static_cast<const T*>(x), ld_x, rt, static_cast<const uint8_t*>(w1), w1s, M, E, K, N, act, tab);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  few_down_kernel<T, F8><<<K / 16, 32 * kDownWarps, (size_t)kDownWarps * M * 16 * 4, st>>>(
-      act, tab, static_cast<const uint8_t*>(w2), w2s, M, rt.topk, K, N, static_cast<T*>(out));
-  return cudaGetLastError();
+  // about 16 warps per SM over all CTAs, so that few rows of output still ask for enough bytes at once
+  const int ctas = K / 16;
+  const int warps = ctas * 6 > num_sms() * 16 ? 4 : ctas * 12 > num_sms() * 16 ? 8 : kDownMaxWarps;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(32 * (unsigned)warps, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)warps * M * 16 * 4;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, few_down_kernel<T, F8>, static_cast<const T*>(act), static_cast<const FewTables*>(tab),
+                            static_cast<const uint8_t*>(w2), w2s, M, rt.topk, K, N, static_cast<T*>(out));
 }
 
 }  // namespace
@@ -480,7 +575,8 @@ extern "C" int moe_few_tokens(int dtype, const void* hidden_states, int64_t ld_h
   const int rc = moe_check_device();
   if (rc != MOE_OK) return rc;
   const FewRouting rt{gating_output, bias,         topk,           renormalize, num_expert_group, topk_group,
-                      scoring_func,  group_score_mode, routed_scaling_factor};
+                      scoring_func,  group_score_mode, routed_scaling_factor,
+                      al16f(gating_output) && (!bias || al16f(bias))};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int M = (int)num_tokens;
   cudaError_t err;
