@@ -11,9 +11,10 @@
 // to fill on that way; a tcgen05 tile would pad 1..8 tokens to a 128-row operand and stage
 // every weight byte through shared memory for the same bytes.
 //
-// The k order inside an MMA is free as long as both operands agree, so a lane takes 32
-// consecutive bytes of its row per 128-byte block (four lanes read one full line) and feeds
-// them to 8 (e4m3) or 4 (16-bit) MMAs in the order they lie. e4m3 codes become fp16 pairs with
+// The k order inside an MMA is free as long as both operands agree, so a lane takes two 16-byte
+// pieces of its row per 128-byte block, 64 bytes apart, and feeds them to 8 (e4m3) or 4 (16-bit)
+// MMAs in the order they lie: the four lanes of a row read 64 bytes in a row at a time, whole 32-byte
+// sectors (32 consecutive bytes per lane asked for every sector twice). e4m3 codes become fp16 pairs with
 // the conversion instruction (moving their bits to bf16 by shifts and masks instead kept the
 // integer pipe busier than HBM: 0.53 against 0.58 of its rate in few_up at one token, 0.53 against
 // 0.64 in few_down at eight), so bf16 tokens and bf16 a_p rows become fp16 too, each row under
@@ -109,13 +110,15 @@ __device__ __forceinline__ float row_scale(uint32_t amax_bits) {
   return e == 0 || e == 255 ? 1.0f : __int_as_float(min(max(127 + 14 - (e - 127), 1), 254) << 23);
 }
 
-// The tokens' side of one k block: 32 or 16 consecutive values of this lane's column, zeros without one.
+// The tokens' side of one k block: this lane's 32 or 16 values of its column, zeros without one.
 // With e4m3 weights the values are wanted in fp16: bf16 ones are scaled and converted.
 template <typename T, bool F8>
 __device__ __forceinline__ void load_col(const T* p, float scale, uint32_t (&x)[F8 ? 16 : 8]) {
+  constexpr int kPart = F8 ? 2 : 1;  // 16-byte pieces that belong to 16 bytes of weights
 #pragma unroll
-  for (int i = 0; i < (F8 ? 4 : 2); ++i) {
-    uint4 v = p ? *reinterpret_cast<const uint4*>(p + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < 2 * kPart; ++i) {
+    const uint4 v = p ? *reinterpret_cast<const uint4*>(p + (i / kPart) * (F8 ? 64 : 32) + (i % kPart) * 8)
+                      : make_uint4(0u, 0u, 0u, 0u);
     x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
   }
   if constexpr (F8 && ElemTraits<T>::kFmt == 1) {
@@ -127,7 +130,7 @@ __device__ __forceinline__ void load_col(const T* p, float scale, uint32_t (&x)[
   }
 }
 
-// One 128-byte k block: rows lo (A rows 0-7) and hi (A rows 8-15), 32 bytes each per lane.
+// One 128-byte k block: rows lo (A rows 0-7) and hi (A rows 8-15), two 16-byte pieces each per lane.
 template <typename T, bool F8>
 __device__ __forceinline__ void block_mma(float (&c)[4], const uint4 (&lo)[2], const uint4 (&hi)[2],
                                           const uint32_t (&x)[F8 ? 16 : 8]) {
@@ -259,7 +262,7 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
 
   constexpr int kElt = F8 ? 1 : 2;                // weight bytes per element
   constexpr int kBlkElts = kBlkBytes / kElt;      // elements of a k block
-  constexpr int kColElts = kBlkElts / 4;          // of them per lane
+  constexpr int kColElts = kBlkElts / 8;          // of them in a lane's 16 bytes
   constexpr int kDepth = 3;                       // k blocks in flight per lane
   const int g = lane >> 2, t4 = lane & 3;
   const int nkb = K / kBlkElts;
@@ -275,7 +278,7 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
   auto row_of = [&](int it) {
     const int64_t i = i0 + it;
     const int c = (int)(i / NB), n0 = (int)(i - (int64_t)c * NB) * 8;
-    return w1 + ((int64_t)s.chunk_expert[c] * 2 * N + n0 + g) * row_bytes + t4 * 32;
+    return w1 + ((int64_t)s.chunk_expert[c] * 2 * N + n0 + g) * row_bytes + t4 * 16;
   };
   const int64_t up = (int64_t)N * row_bytes;
   int l_it = b0 / nkb, l_k = b0 - l_it * nkb, left = b1 - b0;  // the next block to load
@@ -284,9 +287,9 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
   auto load = [&](int d) {
     const uint8_t* p = lp + (int64_t)l_k * kBlkBytes;
     lo[d][0] = ldg_stream(p);
-    lo[d][1] = ldg_stream(p + 16);
+    lo[d][1] = ldg_stream(p + 64);
     hi[d][0] = ldg_stream(p + up);
-    hi[d][1] = ldg_stream(p + up + 16);
+    hi[d][1] = ldg_stream(p + up + 64);
     --left;
     if (++l_k == nkb) {
       l_k = 0;
@@ -397,7 +400,7 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
   constexpr bool kToHalf = F8 && ElemTraits<T>::kFmt == 1;
   constexpr int kElt = F8 ? 1 : 2;
   constexpr int kBlkElts = kBlkBytes / kElt;
-  constexpr int kColElts = kBlkElts / 4;
+  constexpr int kColElts = kBlkElts / 8;
   constexpr int kDepth = 3;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
@@ -412,15 +415,15 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
   const int b0 = (int)((int64_t)total * warp / warps), b1 = (int)((int64_t)total * (warp + 1) / warps);
 
   int lc = b0 / nkb, lk = b0 - lc * nkb, left = b1 - b0;  // the next block to load
-  auto row_of = [&](int c) { return w2 + ((int64_t)tab->chunk_expert[c] * K + h0 + g) * row_bytes + t4 * 32; };
+  auto row_of = [&](int c) { return w2 + ((int64_t)tab->chunk_expert[c] * K + h0 + g) * row_bytes + t4 * 16; };
   const uint8_t* lp = left > 0 ? row_of(lc) : nullptr;
   uint4 lo[kDepth][2], hi[kDepth][2];
   auto load = [&](int d) {
     const uint8_t* p = lp + (int64_t)lk * kBlkBytes;
     lo[d][0] = ldg_stream(p);
-    lo[d][1] = ldg_stream(p + 16);
+    lo[d][1] = ldg_stream(p + 64);
     hi[d][0] = ldg_stream(p + 8 * row_bytes);
-    hi[d][1] = ldg_stream(p + 8 * row_bytes + 16);
+    hi[d][1] = ldg_stream(p + 8 * row_bytes + 64);
     --left;
     if (++lk == nkb) {
       lk = 0;
