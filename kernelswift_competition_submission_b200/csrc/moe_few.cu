@@ -47,6 +47,7 @@ constexpr int kFewMaxTokens = 32;
 constexpr int kFewMaxPairs = 512;
 constexpr int kFewCols = 8;          // pairs per chunk: the MMA's columns
 constexpr int kUpWarps = 12;
+constexpr size_t kUpMaxSmem = 200 * 1024;
 constexpr int kBlkBytes = 128;       // weight bytes of a row per k block
 
 // Written by few_up's first CTA for few_down.
@@ -146,6 +147,15 @@ __device__ __forceinline__ void block_mma(float (&c)[4], const uint4 (&lo)[2], c
   }
 }
 
+// The same from tokens already in fp16.
+__device__ __forceinline__ void load_col16(const __half* p, uint32_t (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 v = p ? *reinterpret_cast<const uint4*>(p + (i / 2) * 64 + (i % 2) * 8) : make_uint4(0u, 0u, 0u, 0u);
+    x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+  }
+}
+
 // The routing of one token by one warp, as moe_grouped_topk does it.
 __device__ __forceinline__ void route_one(const FewRouting& r, int tok, int E, float* w, int32_t* ids,
                                           float* s_choice, RouteScratch* scr) {
@@ -181,6 +191,7 @@ struct UpShared {
   int32_t chunk_expert[kFewMaxPairs];
   int16_t chunk_pair[kFewMaxPairs][kFewCols];
   float scale[kFewMaxTokens];        // by token, e4m3 weights and bf16 tokens
+  uint32_t amax[kFewMaxTokens];
   int32_t n_chunks;
   alignas(16) float part[kUpWarps][2][32][4];  // a warp's sums of an item that it did not begin / did not end
 };
@@ -188,32 +199,56 @@ struct UpShared {
 template <typename T, bool F8>
 __global__ void __launch_bounds__(32 * kUpWarps, 1)
 few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_t* __restrict__ w1,
-              const float* __restrict__ w1s, int M, int E, int K, int N, T* __restrict__ act, FewTables* tab) {
+              const float* __restrict__ w1s, int M, int E, int K, int N, bool staged, T* __restrict__ act, FewTables* tab) {
   extern __shared__ __align__(16) uint8_t smem_up[];
   UpShared& s = *reinterpret_cast<UpShared*>(smem_up);
   constexpr bool kToHalf = F8 && ElemTraits<T>::kFmt == 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int P = M * rt.topk;
+  // few tokens are converted once per CTA into shared memory (pitch: 16 bytes more than a row, so that the
+  // lanes of two columns take different banks); more of them at every use
+  __half* xh = reinterpret_cast<__half*>(smem_up + sizeof(UpShared));
+  const int xh_ld = K + 8;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int t = warp; t < M; t += kUpWarps) {
-    route_one(rt, t, E, s.weight, s.id, s.choice[warp], &s.scratch[warp]);
-    __syncwarp();
-    if constexpr (kToHalf) {
+  if constexpr (kToHalf) {
+    if (threadIdx.x < M) s.amax[threadIdx.x] = 0u;
+    __syncthreads();
+    for (int t = 0; t < M; ++t) {
       uint32_t m = 0;
-      for (int i = lane * 8; i < K; i += 256) {
+      for (int i = threadIdx.x * 8; i < K; i += blockDim.x * 8) {
         const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)t * ld_x + i);
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) m = max(m, max(w[j] << 16 & 0x7FFF0000u, w[j] & 0x7FFF0000u));
       }
       m = __reduce_max_sync(0xffffffffu, m);
-      if (lane == 0) s.scale[t] = row_scale(m);
+      if (lane == 0 && m) atomicMax(&s.amax[t], m);
     }
+  }
+  for (int t = warp; t < M; t += kUpWarps) {
+    route_one(rt, t, E, s.weight, s.id, s.choice[warp], &s.scratch[warp]);
+    __syncwarp();
   }
   for (int i = threadIdx.x; i < E; i += blockDim.x) s.count[i] = 0;
   for (int i = threadIdx.x; i < kFewMaxPairs * kFewCols / 2; i += blockDim.x)
     reinterpret_cast<uint32_t*>(s.chunk_pair)[i] = 0xFFFFFFFFu;
   __syncthreads();
+  if constexpr (kToHalf) {
+    if (threadIdx.x < M) s.scale[threadIdx.x] = row_scale(s.amax[threadIdx.x]);
+    if (staged)
+      for (int t = 0; t < M; ++t) {
+        const float sc = row_scale(s.amax[t]);
+        for (int i = threadIdx.x * 8; i < K; i += blockDim.x * 8) {
+          const uint4 v = *reinterpret_cast<const uint4*>(x + (int64_t)t * ld_x + i);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = ElemTraits<__half>::pack2(__uint_as_float(w[j] << 16) * sc, __uint_as_float(w[j] & 0xFFFF0000u) * sc);
+          *reinterpret_cast<uint4*>(xh + t * xh_ld + i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+  }
   for (int p = threadIdx.x; p < P; p += blockDim.x)
     if (s.id[p] >= 0 && s.id[p] < E) atomicAdd(&s.count[s.id[p]], 1);
   __syncthreads();
@@ -305,6 +340,7 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
   bool begun = kb == 0;  // this warp has the item from its first block on
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const T* xp = nullptr;
+  const __half* hp = nullptr;
   float xs = 1.0f;
   const float* sg = nullptr;
   const float* su = nullptr;
@@ -313,7 +349,10 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
     const int c = (int)(i / NB), n0 = (int)(i - (int64_t)c * NB) * 8;
     const int pair = s.chunk_pair[c][g];
     xp = pair >= 0 ? x + (int64_t)(pair / rt.topk) * ld_x + t4 * kColElts : nullptr;
-    if constexpr (kToHalf) xs = pair >= 0 ? s.scale[pair / rt.topk] : 1.0f;
+    if constexpr (kToHalf) {
+      xs = pair >= 0 ? s.scale[pair / rt.topk] : 1.0f;
+      hp = pair >= 0 ? xh + (pair / rt.topk) * xh_ld + t4 * kColElts : nullptr;
+    }
     if constexpr (F8) {
       sg = w1s + ((int64_t)s.chunk_expert[c] * (2 * N / 128) + n0 / 128) * (K / 128);
       su = sg + (int64_t)(N / 128) * (K / 128);
@@ -349,7 +388,14 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
     for (int d = 0; d < kDepth; ++d) {
       if (b + d < b1) {
         uint32_t xv[F8 ? 16 : 8];
-        load_col<T, F8>(xp ? xp + (int64_t)kb * kBlkElts : nullptr, xs, xv);
+        bool have = false;
+        if constexpr (kToHalf) {
+          if (staged) {
+            load_col16(hp ? hp + kb * kBlkElts : nullptr, xv);
+            have = true;
+          }
+        }
+        if (!have) load_col<T, F8>(xp ? xp + (int64_t)kb * kBlkElts : nullptr, xs, xv);
         if constexpr (F8) {
           float part[4] = {0.f, 0.f, 0.f, 0.f};
           block_mma<T, F8>(part, lo[d], hi[d], xv);
@@ -516,14 +562,17 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
                        cudaStream_t st) {
   FewTables* tab = static_cast<FewTables*>(ws);
   T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(ws) + few_tables_bytes());
-  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(few_up_kernel<T, F8>), (int)sizeof(UpShared));
+  const size_t rows = (size_t)M * (size_t)(K + 8) * 2;
+  const bool staged = F8 && ElemTraits<T>::kFmt == 1 && sizeof(UpShared) + rows <= kUpMaxSmem;
+  const size_t smem = sizeof(UpShared) + (staged ? rows : 0);
+  cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(few_up_kernel<T, F8>), (int)smem);
   if (err != cudaSuccess) return err;
   if (F8 && ElemTraits<T>::kFmt == 1) {
     err = cudaMemsetAsync(tab->amax, 0, sizeof(uint32_t) * (size_t)M * rt.topk, st);
     if (err != cudaSuccess) return err;
   }
-  few_up_kernel<T, F8><<<num_sms(), 32 * kUpWarps, sizeof(UpShared), st>>>(
-      static_cast<const T*>(x), ld_x, rt, static_cast<const uint8_t*>(w1), w1s, M, E, K, N, act, tab);
+  few_up_kernel<T, F8><<<num_sms(), 32 * kUpWarps, smem, st>>>(
+      static_cast<const T*>(x), ld_x, rt, static_cast<const uint8_t*>(w1), w1s, M, E, K, N, staged, act, tab);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
   // about 16 warps per SM over all CTAs, so that few rows of output still ask for enough bytes at once
   const int ctas = K / 16;
