@@ -390,6 +390,23 @@ __device__ __forceinline__ bool named_bar_and(int id, int threads, bool pred) {
   return r != 0;
 }
 
+// ---------------------------------------------------------------- pairs of fp32
+// (a0, a1) * (m, m) + (c, c) and (a0, a1) + (b0, b1) in one instruction each.
+__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float m, float c) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add_pair(float& d0, float& d1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(b0), "f"(b1));
+}
+
 // ---------------------------------------------------------------- element types
 template <typename T> struct ElemTraits;
 template <> struct ElemTraits<__nv_bfloat16> {

@@ -281,73 +281,77 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     int kslot = 0, vslot = 3;  // ring position of the tile's K (three slots) and V (two)
     uint32_t kphase = 0, vphase = 0;
     auto at = [](int s) { return s >= kPfSlots ? s - kPfSlots : s; };
-    auto wait_slots = [&](int s0, int n, uint32_t ph) {
-      for (int c = 0; c < n; ++c)
-        ok = mbar_wait_warp(&full[at(s0 + c)], s0 + c >= kPfSlots ? ph ^ 1 : ph, a.status, s_abort) && ok;
-      tc_fence_after();
-    };
-    // S of subtile i from the K at kslot; `last`: no later user of this K
+    // one lane issues: S of subtile i from the K at kslot; `last`: no later user of this K
     auto issue_qk = [&](int i, bool last) {
-      if (one) {
 #pragma unroll
-        for (int c = 0; c < 3; ++c) {
-          const uint64_t da = dq0 + i * (kQSubBytes >> 4) + c * (16384 >> 4);
-          const uint64_t db = dk0 + (uint32_t)at(kslot + c) * (kSlotBytes >> 4);
+      for (int c = 0; c < 3; ++c) {
+        const uint64_t da = dq0 + i * (kQSubBytes >> 4) + c * (16384 >> 4);
+        const uint64_t db = dk0 + (uint32_t)at(kslot + c) * (kSlotBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tmem + i * 128, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
-        }
-        umma_commit(&s_full[i]);
-        if (last)
-          for (int c = 0; c < 3; ++c) umma_commit(&empty[at(kslot + c)]);
+        for (int k = 0; k < 4; ++k) umma_f16(tmem + i * 128, da + 2 * k, db + 2 * k, kIdescQK, (c | k) != 0);
       }
-      __syncwarp();
+      umma_commit(&s_full[i]);
+      if (last)
+        for (int c = 0; c < 3; ++c) umma_commit(&empty[at(kslot + c)]);
     };
     auto issue_pv = [&](int i, bool first, bool fin, bool last) {
-      if (one) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint64_t db = dv0 + (uint32_t)at(vslot + c) * (kSlotBytes >> 4);
+      for (int c = 0; c < 2; ++c) {
+        const uint64_t db = dv0 + (uint32_t)at(vslot + c) * (kSlotBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (c * 4 + k) * 8, db + 128 * k, kIdescPV,
-                        !first || (c | k) != 0);
-        }
-        if (fin) umma_commit(&o_full[i]);
-        if (last)
-          for (int c = 0; c < 2; ++c) umma_commit(&empty[at(vslot + c)]);
+        for (int k = 0; k < 4; ++k)
+          umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (c * 4 + k) * 8, db + 128 * k, kIdescPV,
+                      !first || (c | k) != 0);
       }
-      __syncwarp();
+      if (fin) umma_commit(&o_full[i]);
+      if (last)
+        for (int c = 0; c < 2; ++c) umma_commit(&empty[at(vslot + c)]);
     };
     auto forward = [&](int& s, uint32_t& ph) {
       s += 5;
       if (s >= kPfSlots) { s -= kPfSlots; ph ^= 1; }
     };
-    // a wait that gave up ends the loop at the next tile; until then the MMAs run on what is there
+    // Everything that PV of a subtile and its next QK need is waited for at once (a wait costs about 125 clocks
+    // when all is there, and a subtile's softmax, PV and QK are one chain): lanes 0-1 V, 2 its check, 3 P, 4-6 K.
+    // A wait that gave up ends the loop at the next tile; until then the MMAs run on what is there.
+    auto wait_all = [&](int j, int i, bool pv, bool qk) {
+      uint64_t* bar = nullptr;
+      uint32_t ph = 0;
+      if (pv && lane < 2) {
+        bar = &full[at(vslot + lane)];
+        ph = vslot + lane >= kPfSlots ? vphase ^ 1 : vphase;
+      } else if (pv && lane == 2) {
+        bar = &v_ok[j & 1];
+        ph = (j >> 1) & 1;
+      } else if (pv && lane == 3) {
+        bar = &p_full[i];
+        ph = j & 1;
+      } else if (qk && lane >= 4 && lane < 7) {
+        bar = &full[at(kslot + lane - 4)];
+        ph = kslot + lane - 4 >= kPfSlots ? kphase ^ 1 : kphase;
+      }
+      ok = mbar_wait_lanes(bar, ph, a.status, s_abort) && ok;
+      tc_fence_after();
+    };
     ok = mbar_wait_warp(q_full, 0, a.status, s_abort);
-    wait_slots(0, 3, 0);
-    if (n_tiles[0] > 0) issue_qk(0, n_tiles[1] == 0);
-    if (n_tiles[1] > 0) issue_qk(1, true);
+    wait_all(0, 0, false, true);
+    if (one) {
+      if (n_tiles[0] > 0) issue_qk(0, n_tiles[1] == 0);
+      if (n_tiles[1] > 0) issue_qk(1, true);
+    }
+    __syncwarp();
     forward(kslot, kphase);
     for (int j = 0; j < n_max && ok; ++j) {
-      bool v_here = false, k_here = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (j < n_tiles[i]) {
-          if (!v_here) {
-            wait_slots(vslot, 2, vphase);
-            ok = mbar_wait_warp(&v_ok[j & 1], (j >> 1) & 1, a.status, s_abort) && ok;
-            v_here = true;
+        const bool pv = j < n_tiles[i], qk = j + 1 < n_tiles[i];
+        if (pv || qk) {
+          wait_all(j, i, pv, qk);
+          if (one) {
+            if (pv) issue_pv(i, j == 0, j + 1 == n_tiles[i], i == 1 || n_tiles[1] <= j);
+            if (qk) issue_qk(i, i == 1 || n_tiles[1] <= j + 1);
           }
-          ok = mbar_wait_warp(&p_full[i], j & 1, a.status, s_abort) && ok;
-          tc_fence_after();
-          issue_pv(i, j == 0, j + 1 == n_tiles[i], i == 1 || n_tiles[1] <= j);
-        }
-        if (j + 1 < n_tiles[i]) {
-          if (!k_here) {
-            wait_slots(kslot, 3, kphase);
-            k_here = true;
-          }
-          issue_qk(i, i == 1 || n_tiles[1] <= j + 1);
+          __syncwarp();
         }
       }
       forward(vslot, vphase);
@@ -431,7 +435,8 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[c][x]));
+        for (int x = 0; x < 32; x += 2)
+          mx[(x >> 1) & 3] = fmaxf(fmaxf(mx[(x >> 1) & 3], __uint_as_float(raw[c][x])), __uint_as_float(raw[c][x + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
       const bool move = top > m_ref + kRescaleLog2 || m_ref == -INFINITY;
       float f = 1.0f;
@@ -461,10 +466,12 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
           const int e = c * 64 + 2 * x;
-          const float p0 = ex2(fmaf(__uint_as_float(raw[e >> 5][e & 31]), a.scale_log2, -base));
-          const float p1 = ex2(fmaf(__uint_as_float(raw[e >> 5][(e & 31) + 1]), a.scale_log2, -base));
-          sum[x & 1] += p0;
-          sum[2 + (x & 1)] += p1;
+          float p0, p1;
+          fma_pair(p0, p1, __uint_as_float(raw[e >> 5][e & 31]), __uint_as_float(raw[e >> 5][(e & 31) + 1]),
+                   a.scale_log2, -base);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          add_pair(sum[2 * (x & 1)], sum[2 * (x & 1) + 1], p0, p1);
           p[x] = ElemTraits<T>::pack2(p0, p1);
         }
         tmem_st32(t_s + c * 32, p);
