@@ -5,13 +5,14 @@
 //
 // One CTA takes 256 query rows of one head as two 128-row subtiles and walks the keys 128 at a
 // time with a running maximum and sum per row:
-//   warps 0-3, 4-7  softmax of subtile 0 / 1, one row per thread: S from TMEM into registers,
-//                   maximum, exp2, row sum in fp32, P as 16-bit pairs back into S's columns
-//   warp 8          TMA producer: K as three [128 keys][64] boxes, V as two [64 keys][128] halves,
+//   warps 0-7, 8-15 softmax of subtile 0 / 1, two threads per row with 64 keys each: S from TMEM into
+//                   registers, maximum, exp2, row sum in fp32, P as 16-bit pairs back into S's columns
+//                   (one thread per row with 128 keys took 2100 clocks of a chain of 4200 per tile)
+//   warp 16         TMA producer: K as three [128 keys][64] boxes, V as two [64 keys][128] halves,
 //                   16 KB slots in a ring of 8, in the order the MMAs use them
-//   warp 9          MMA issuer: S = Q K^T from shared memory, O += P V with P from TMEM and V as it
+//   warp 17         MMA issuer: S = Q K^T from shared memory, O += P V with P from TMEM and V as it
 //                   lies (MN-major)
-//   warps 10-11     look at V before its MMAs where a row of the tile may not see a key (see below)
+//   warps 18-19     look at V before its MMAs where a row of the tile may not see a key (see below)
 // The MMAs of one subtile run while the other one's softmax does: after PV of subtile i the next
 // QK of i is issued at once, so its scores wait for the softmax and not the other way round.
 //
@@ -21,7 +22,7 @@
 // inputs' type for the second product (as wide as V itself); l sums the unrounded values.
 //
 // Masked places: a score is replaced before the maximum is taken, so keys may hold anything.
-// V meets P = 0 in the MMA, and 0 * NaN is NaN, so warps 10-11 zero the V rows past the request's
+// V meets P = 0 in the MMA, and 0 * NaN is NaN, so warps 18-19 zero the V rows past the request's
 // end, and look for non-finite values in tiles that some row sees only in part; if there is one,
 // the CTA's rows are computed again by the softmax warps, key by key over visible keys only.
 //
@@ -32,7 +33,8 @@
 namespace moe {
 namespace {
 
-constexpr int kPfThreads = 384;
+constexpr int kPfSoftmax = 256;          // softmax threads of a subtile
+constexpr int kPfThreads = 2 * kPfSoftmax + 128;
 constexpr int kPfTile = 128;             // keys per tile, rows per subtile
 constexpr int kPfSlots = 8;
 constexpr int kSlotBytes = 16384;
@@ -41,7 +43,8 @@ constexpr float kRescaleLog2 = 8.0f;
 
 struct PfSmem {
   static constexpr int kRing = 2 * kQSubBytes;
-  static constexpr int kBars = kRing + kPfSlots * kSlotBytes;
+  static constexpr int kX = kRing + kPfSlots * kSlotBytes;  // the row's threads' maxima (bf16) or sums
+  static constexpr int kBars = kX + 1024;
   // q, full[8], empty[8], s_full[2], p_full[2], o_full[2], v_ok[2], mma_done
   static constexpr int kNumBars = 1 + 2 * kPfSlots + 9;
   static constexpr int kMisc = kBars + kNumBars * 8;
@@ -171,10 +174,10 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
     if (lane == 0) { s_unit[0] = found; s_unit[1] = tile; }
   }
-  if (threadIdx.x == 64) {
+  if (threadIdx.x == 32) {
     mbar_init(q_full, 1);
     for (int s = 0; s < kPfSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kPfSoftmax); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); }
     mbar_init(mma_done, 1);
     *s_abort = 0;
     *s_bad = 0;
@@ -208,12 +211,12 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int sure = min(nk, a.causal ? max(0, nk - nq + 1 + row0) : nk) / kPfTile;  // tiles all rows see whole
 
   if (n_max > 0) {
-    if (warp == 9) { tmem_alloc(s_tmem, 512); tmem_relinquish(); }
+    if (warp == 17) { tmem_alloc(s_tmem, 512); tmem_relinquish(); }
     tc_fence_before();
   }
   __syncthreads();
   if (n_max == 0) {
-    if (warp < 8) {
+    if (warp < 8) {  // 256 rows
       const int i = row0 + threadIdx.x;
       if (i < nq) {
         const int64_t row = (q_lo + i) * a.heads + h;
@@ -228,7 +231,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ------------------------------------------------ TMA producer: the warp converged, one lane issues
     const bool one = elect_one();
     if (one) {
@@ -271,7 +274,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       for (int s = 0; s < kPfSlots; ++s)
         if ((issued >> s) & 1u) mbar_wait_warp(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ------------------------------------------------ MMA issuer: the warp converged, one lane issues
     constexpr uint32_t kIdescQK = idesc_f16(128, 128, ElemTraits<T>::kFmt);
     constexpr uint32_t kIdescPV = idesc_f16(128, 128, ElemTraits<T>::kFmt) | kIdescBMnMajor;
@@ -360,11 +363,11 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (one) umma_commit(mma_done);  // every MMA issued here is done before TMEM is freed
     __syncwarp();
     mbar_wait_warp(mma_done, 0, nullptr, nullptr);
-  } else if (warp >= 10) {
+  } else if (warp >= 18) {
     // ------------------------------------------------ V where a row may not see a key
     // They pass every tile on (v_ok, two in turn: the ring holds no more than two tiles' V), so
     // they see each phase of the ring's barriers.
-    const int vt = threadIdx.x - 320;  // 0 .. 63: a key row of each half
+    const int vt = threadIdx.x - (2 * kPfSoftmax + 64);  // 0 .. 63: a key row of each half
     bool ok = true;
     for (int j = 0; j < n_max && ok; ++j) {
       bool wrote = false;
@@ -401,43 +404,53 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (ok) mbar_arrive(&v_ok[j & 1]);
     }
   } else {
-    // ------------------------------------------------ softmax, one row per thread
-    const int sub = warp >> 2;
-    const int i_row = row0 + threadIdx.x;  // row of the request
+    // ------------------------------------------------ softmax, two threads per row
+    const int sub = warp >> 3, half = (warp >> 2) & 1;   // keys 64 half .. + 63 of S, values 64 half .. + 63 of O
+    const int r = (warp & 3) * 32 + lane;                // row of the subtile
+    const int i_row = row0 + sub * kPfTile + r;          // row of the request
     const int limit = seen(i_row);
     const int n_t = n_tiles[sub];
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // 32 lanes per warp
-    const uint32_t t_s = lane_base + sub * 128, t_o = lane_base + 256 + sub * 128;
+    const uint32_t t_s = lane_base + sub * 128, t_o = lane_base + 256 + sub * 128 + half * 64;
+    __nv_bfloat16* x_max = reinterpret_cast<__nv_bfloat16*>(smem + PfSmem::kX) + sub * kPfSoftmax;
+    float* x_sum = reinterpret_cast<float*>(smem + PfSmem::kX) + sub * kPfTile;
+    const int x_me = half * kPfTile + r;
     float m_ref = -INFINITY, l = 0.f;  // in log2 units of the scaled scores
     bool ok = true;
     for (int j = 0; j < n_t; ++j) {
-      if (!mbar_wait(&s_full[sub], j & 1, a.status, s_abort)) { ok = false; break; }
+      // a wait that gave up is carried to the next barrier of the subtile's warps, so that all leave together
+      ok = mbar_wait(&s_full[sub], j & 1, a.status, s_abort) && ok;
       tc_fence_after();
-      uint32_t raw[4][32];
+      uint32_t raw[2][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, raw[c]);
+      for (int c = 0; c < 2; ++c) tmem_ld32(t_s + half * 64 + c * 32, raw[c]);
       tmem_wait_ld();
       if (a.neg) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int x = 0; x < 32; ++x) raw[c][x] ^= 0x80000000u;
       }
-      const int vis = limit - j * kPfTile;  // keys of this tile that the row sees
-      if (__any_sync(0xffffffffu, vis < kPfTile)) {
+      const int vis = limit - j * kPfTile - half * 64;  // of this thread's keys, those that the row sees
+      if (__any_sync(0xffffffffu, vis < 64)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int x = 0; x < 32; ++x)
             if (c * 32 + x >= vis) raw[c][x] = 0xFF800000u;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int x = 0; x < 32; x += 2)
           mx[(x >> 1) & 3] = fmaxf(fmaxf(mx[(x >> 1) & 3], __uint_as_float(raw[c][x])), __uint_as_float(raw[c][x + 1]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      // Any common reference near the row's maximum will do: its two threads exchange theirs rounded up to bf16.
+      // The place is free: this tile's scores follow the P that every thread gave after it had read the last ones.
+      x_max[x_me] = __float2bfloat16_ru(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      ok = named_bar_and(1 + sub, kPfSoftmax, ok);
+      if (!ok) break;
+      const float top = fmaxf(__bfloat162float(x_max[r]), __bfloat162float(x_max[kPfTile + r])) * a.scale_log2;
       const bool move = top > m_ref + kRescaleLog2 || m_ref == -INFINITY;
       float f = 1.0f;
       if (move) {
@@ -450,59 +463,67 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const float g = move ? f : 1.0f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + c * 32, o);
+          uint32_t o[16];
+          tmem_ld16(t_o + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * g);
-          tmem_st32(t_o + c * 32, o);
+          for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * g);
+          tmem_st16(t_o + c * 16, o);
         }
       }
       const float base = m_ref == -INFINITY ? 0.f : m_ref;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      // P takes the place of S's first 64 columns, which the row's other thread has read before the barrier
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
+        uint32_t p[16];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const int e = c * 64 + 2 * x;
+        for (int x = 0; x < 16; ++x) {
           float p0, p1;
-          fma_pair(p0, p1, __uint_as_float(raw[e >> 5][e & 31]), __uint_as_float(raw[e >> 5][(e & 31) + 1]),
-                   a.scale_log2, -base);
+          fma_pair(p0, p1, __uint_as_float(raw[c][2 * x]), __uint_as_float(raw[c][2 * x + 1]), a.scale_log2, -base);
           p0 = ex2(p0);
           p1 = ex2(p1);
           add_pair(sum[2 * (x & 1)], sum[2 * (x & 1) + 1], p0, p1);
           p[x] = ElemTraits<T>::pack2(p0, p1);
         }
-        tmem_st32(t_s + c * 32, p);
+        tmem_st16(t_s + half * 32 + c * 16, p);
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[sub]);
     }
-    if (n_t > 0 && ok) ok = mbar_wait(&o_full[sub], 0, a.status, s_abort);
+    if (n_t > 0) ok = mbar_wait(&o_full[sub], 0, a.status, s_abort) && ok;
     tc_fence_after();
+    ok = named_bar_and(1 + sub, kPfSoftmax, ok);  // the last maxima are read
+    if (half == 1) x_sum[r] = l;
+    named_bar_sync(1 + sub, kPfSoftmax);
+    if (half == 0) {
+      l += x_sum[r];
+      x_sum[r] = l;
+    }
+    named_bar_sync(1 + sub, kPfSoftmax);
+    l = x_sum[r];
     const bool live = i_row < nq;
     const int64_t row = (q_lo + i_row) * a.heads + h;
     if (*s_bad) {
       if (ok)
-        for (int r = 0; r < 32; ++r) {
-          const int i = row0 + warp * 32 + r;
+        for (int rr = warp & 7; rr < kPfTile; rr += kPfSoftmax / 32) {
+          const int i = row0 + sub * kPfTile + rr;
           if (i < nq) prefill_row<T>(a, q_lo + i, h, k_lo, seen(i));
         }
     } else {
       const bool some = l > 0.f || l != l;
       const float inv = some ? 1.0f / l : 0.f;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t o[32];
         if (n_t > 0) {
           tmem_ld32(t_o + c * 32, o);
           tmem_wait_ld();
         }
         if (live) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * kNopeDim + c * 32);
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * kNopeDim + half * 64 + c * 32);
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             uint32_t w[4];
@@ -515,12 +536,13 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           }
         }
       }
-      if (live && a.lse != nullptr) a.lse[row] = some ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      if (live && half == 0 && a.lse != nullptr)
+        a.lse[row] = some ? (m_ref + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     __syncwarp();
     tmem_dealloc(tmem, 512);
