@@ -40,6 +40,8 @@ constexpr int kPfSlots = 8;
 constexpr int kSlotBytes = 16384;
 constexpr int kQSubBytes = 3 * 16384;    // a subtile of Q: three [128 rows][64] chunks
 constexpr float kRescaleLog2 = 8.0f;
+constexpr int kPolyEvery = 4;  // every second pair of exponentials by polynomial: the exponential units alone take
+                               // 1024 clocks per subtile and tile of a chain of 4400
 
 struct PfSmem {
   static constexpr int kRing = 2 * kQSubBytes;
@@ -76,6 +78,30 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x of two values x <= 2^7 without the exponential unit: x = n + f with n the nearest integer, 2^f by its
+// degree-4 polynomial of least relative error on [-1/2, 1/2] (2.7e-6 in fp32; a weighted least-squares fit at
+// Chebyshev nodes iterated to equal extrema), times 2^n made from n's bits. n stops at -127, whose bits are
+// those of zero: -inf and everything below 2^-126 give 0, NaN stays NaN.
+__device__ __forceinline__ void exp2_poly_pair(float& y0, float& y1, float x0, float x1) {
+  asm("{\n\t.reg .f32 a, b, c, d;\n\t.reg .b32 m, n;\n\t.reg .b64 x, t, f, p, k, s;\n\t"
+      "max.NaN.f32 a, %2, 0fC2FE0000;\n\tmax.NaN.f32 b, %3, 0fC2FE0000;\n\t"  // -127
+      "mov.b64 x, {a, b};\n\t"
+      "mov.b64 k, 0x4B4000004B400000;\n\tadd.rn.f32x2 t, x, k;\n\t"            // 1.5 * 2^23: n in the low bits
+      "mov.b64 {m, n}, t;\n\t"
+      "mov.b64 k, 0xCB400000CB400000;\n\tadd.rn.f32x2 f, t, k;\n\t"
+      "mov.b64 k, 0xBF800000BF800000;\n\tfma.rn.f32x2 f, f, k, x;\n\t"         // f = x - n
+      "mov.b64 {c, d}, f;\n\t"
+      "mov.b64 p, {%4, %4};\n\tmov.b64 k, {%5, %5};\n\tfma.rn.f32x2 p, p, f, k;\n\t"
+      "mov.b64 k, {%6, %6};\n\tfma.rn.f32x2 p, p, f, k;\n\t"
+      "mov.b64 k, {%7, %7};\n\tfma.rn.f32x2 p, p, f, k;\n\t"
+      "mov.b64 k, {%8, %8};\n\tfma.rn.f32x2 p, p, f, k;\n\t"
+      "shl.b32 m, m, 23;\n\tadd.s32 m, m, 0x3F800000;\n\tshl.b32 n, n, 23;\n\tadd.s32 n, n, 0x3F800000;\n\t"
+      "mov.b64 s, {m, n};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(y0), "=f"(y1)
+      : "f"(x0), "f"(x1), "f"(0.009570101276040077f), "f"(0.05591785907745361f), "f"(0.240247443318367f),
+        "f"(0.6931217908859253f), "f"(0.9999992847442627f));
 }
 
 // One row by a warp, key by key, over the keys it sees: fp32, online softmax. Lane l holds
@@ -481,8 +507,12 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int x = 0; x < 16; ++x) {
           float p0, p1;
           fma_pair(p0, p1, __uint_as_float(raw[c][2 * x]), __uint_as_float(raw[c][2 * x + 1]), a.scale_log2, -base);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
+          if (x % kPolyEvery == kPolyEvery - 1) {
+            exp2_poly_pair(p0, p1, p0, p1);
+          } else {
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+          }
           add_pair(sum[2 * (x & 1)], sum[2 * (x & 1) + 1], p0, p1);
           p[x] = ElemTraits<T>::pack2(p0, p1);
         }
