@@ -70,7 +70,7 @@ def _table(name: str, block_table: torch.Tensor, num_seqs: int) -> torch.Tensor:
 def _ints(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name}: {what} must be a 1-D int32 or int64 tensor")
-    return t.to(torch.int32).contiguous()
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
 def latent_cache_write(cache: torch.Tensor, latent: torch.Tensor, k_rope: torch.Tensor, slots: torch.Tensor) -> None:
@@ -91,7 +91,8 @@ def latent_cache_write(cache: torch.Tensor, latent: torch.Tensor, k_rope: torch.
         raise ValueError(f"{name}: latent, k_rope and slots must have the same number of rows")
     if slots.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name}: slots must be int32 or int64")
-    slots = slots.to(torch.int64).contiguous()
+    if slots.dtype != torch.int64 or slots.stride(0) != 1:
+        slots = slots.to(torch.int64).contiguous()
     _lib.check(
         _lib.load().moe_latent_cache_write(_DTYPES[want], _ptr(latent), latent.stride(0), _ptr(k_rope),
                                            k_rope.stride(0), _ptr(slots), n, fmt, _ptr(cache), cache.shape[0],

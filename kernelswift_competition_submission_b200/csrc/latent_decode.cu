@@ -927,10 +927,9 @@ latent_decode_join_kernel(const __grid_constant__ DcArgs a) {
 
 constexpr int kMaxDev = 64;
 
-// CTA pairs that can be resident at once (a pair needs two SMs of one cluster); asked once per device.
+// CTA pairs that can be resident at once (a pair needs two SMs of one cluster); asked once per device and kernel.
 template <typename K>
-cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int* pairs) {
-  static int cache[kMaxDev];
+cudaError_t resident_pairs(K kern, cudaLaunchConfig_t cfg, int (&cache)[kMaxDev], int* pairs) {
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
@@ -988,7 +987,8 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if ((err = resident_pairs(kern, cfg, &a.pairs)) != cudaSuccess) return err;
+  static int pairs_of_device[kMaxDev];
+  if ((err = resident_pairs(kern, cfg, pairs_of_device, &a.pairs)) != cudaSuccess) return err;
   cfg.gridDim = dim3(2 * (unsigned)a.pairs, 1, 1);
   if ((err = cudaLaunchKernelEx(&cfg, kern, mq, mc, mr, ms, a)) != cudaSuccess) return err;
   latent_decode_join_kernel<T><<<(unsigned)ceil_div((int64_t)a.num_seqs * a.rows, 4), 128, 0, st>>>(a);

@@ -28,8 +28,7 @@
 //           the number of items; items cut between warps are joined in shared memory in order.
 // few_down: one CTA per 16 rows of the output; its warps take consecutive runs of the (chunk, k
 //           block) list, add weight * product into their own shared rows in fp32, and the rows are
-//           summed in warp order. It is launched while few_up still runs and waits for it on the
-//           device.
+//           summed in warp order.
 // Both give the same bits on every run. Sums are fp32; a_p is rounded once to the tokens' type (the
 // layer's other paths do the same).
 #include "common.cuh"
@@ -209,7 +208,6 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
   // lanes of two columns take different banks); more of them at every use
   __half* xh = reinterpret_cast<__half*>(smem_up + sizeof(UpShared));
   const int xh_ld = K + 8;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if constexpr (kToHalf) {
     if (threadIdx.x < M) s.amax[threadIdx.x] = 0u;
     __syncthreads();
@@ -443,7 +441,7 @@ few_up_kernel(const T* __restrict__ x, int64_t ld_x, FewRouting rt, const uint8_
 
 template <typename T, bool F8, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
-few_down_kernel(const T* act, const FewTables* tab, const uint8_t* __restrict__ w2,
+few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, const uint8_t* __restrict__ w2,
                 const float* __restrict__ w2s, int M, int topk, int K, int N, T* __restrict__ out) {
   extern __shared__ __align__(16) float s_part[];  // [warps][M][16]
   constexpr bool kToHalf = F8 && ElemTraits<T>::kFmt == 1;
@@ -459,9 +457,6 @@ few_down_kernel(const T* act, const FewTables* tab, const uint8_t* __restrict__ 
   float* mine = s_part + warp * M * 16;
   for (int i = lane; i < M * 16; i += 32) mine[i] = 0.f;
   __syncwarp();
-  // few_up's rows and tables, hence no __restrict__ on their pointers: loads of what is known never to change
-  // may move above this
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int total = tab->n_chunks * nkb;
   const int b0 = (int)((int64_t)total * warp / WARPS), b1 = (int)((int64_t)total * (warp + 1) / WARPS);
 
@@ -577,19 +572,10 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
   // about 16 warps per SM over all CTAs, so that few rows of output still ask for enough bytes at once
   const int ctas = K / 16;
   const int warps = ctas * 6 > num_sms() * 16 ? 4 : ctas * 12 > num_sms() * 16 ? 8 : 16;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
-  cfg.blockDim = dim3(32 * (unsigned)warps, 1, 1);
-  cfg.dynamicSmemBytes = (size_t)warps * M * 16 * 4;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   auto kern = warps == 4 ? few_down_kernel<T, F8, 4> : warps == 8 ? few_down_kernel<T, F8, 8> : few_down_kernel<T, F8, 16>;
-  return cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(act), static_cast<const FewTables*>(tab),
-                            static_cast<const uint8_t*>(w2), w2s, M, rt.topk, K, N, static_cast<T*>(out));
+  kern<<<(unsigned)ctas, 32 * warps, (size_t)warps * M * 16 * 4, st>>>(act, tab, static_cast<const uint8_t*>(w2), w2s, M,
+                                                                      rt.topk, K, N, static_cast<T*>(out));
+  return cudaGetLastError();
 }
 
 }  // namespace

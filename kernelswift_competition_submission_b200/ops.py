@@ -33,7 +33,8 @@ def _ptr(t: torch.Tensor | None):
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the stream's handle without a torch.cuda.Stream object around it (2 us less per call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _require_cuda(name: str, *ts: torch.Tensor) -> torch.device:
