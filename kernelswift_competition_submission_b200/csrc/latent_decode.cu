@@ -14,7 +14,7 @@
 //   warps 8, 10 TMA producers of K and of V: 16 KB slots ([64 keys][128 values]), four for a tile's K and four for
 //              its V, the rotary keys in a buffer of their own; each slot is refilled as soon as it has been read
 //   warps 11-26 (e4m3 pages) widen the codes that the TMA left in half of a slot to bf16 over the whole slot
-//              (exact: the scales are powers of two), two warps a slot
+//              (exact: the scales are powers of two), eight warps a slot
 //   warp 9     MMA issuer (first CTA): QK two tiles ahead of PV, so that the softmax of tile j runs
 //              beside PV of j - 1 and QK of j + 1
 //
@@ -52,13 +52,13 @@ struct DcSmem {
   static constexpr int kRing = 9 * 8192;                      // after Q: nine [64 rows][64] chunks
   static constexpr int kRope = kRing + kDcSlots * kDcSlotBytes;  // [64 keys][64]
   static constexpr int kP = kRope + 8192;                     // two [64 rows][64 keys] chunks
-  static constexpr int kX = kP + 16384;                       // the row's threads' maxima (bf16, two tiles) or sums
-  static constexpr int kBars = kX + kDcSoftmax * 4;
+  static constexpr int kX = kP + 16384;                       // the rows' threads' maxima (two tiles) or sums
+  static constexpr int kBars = kX + 2 * kDcSoftmax * 4;
   // full[8], empty[8], raw[8], rope_full, rope_free, q_full, q_free, s_full[2], p_full, pv_done, o_free, mma_done,
   // fix, v_fixed
   static constexpr int kNumBars = 3 * kDcSlots + 12;
   static constexpr int kMisc = kBars + kNumBars * 8;
-  static constexpr int kBytes = kMisc + 64 + 1024;
+  static constexpr int kBytes = kMisc + 64;
 };
 
 struct DcArgs {
@@ -248,8 +248,12 @@ __global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
 latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
                      const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_s,
                      const __grid_constant__ DcArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // the swizzled tiles need 1024 bytes, and there is no room to round a base up
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) record_status(a.status, MOE_ERR_UNSUPPORTED);
+    return;
+  }
   uint8_t* ring = smem + DcSmem::kRing;
   uint8_t* s_p = smem + DcSmem::kP;
   float* s_x = reinterpret_cast<float*>(smem + DcSmem::kX);
@@ -682,7 +686,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       const bool bad_page = *s_badpage == seg + 1;
       for (int j = sg.k0; j < sg.k1; ++j, ++g) {
-        // a wait that gave up is carried to the next barrier of the four warps, so that all leave together
+        // a wait that gave up is carried to the next barrier of the softmax warps, so that all leave together
         ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
         tc_fence_after();
         uint32_t raw[32];
@@ -713,15 +717,14 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int x = 0; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(raw[x]));
-        // the row's other keys are with three other threads. Any common reference near the maximum will do:
-        // they exchange it rounded up to bf16, two tiles' worth in turn
-        __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(s_x) + (g & 1) * kDcSoftmax;
-        x[threadIdx.x] = __float2bfloat16_ru(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        // the row's other keys are with three other threads; two tiles' maxima in turn
+        float* x = s_x + (g & 1) * kDcSoftmax;
+        x[threadIdx.x] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         ok = named_bar_and(1, kDcSoftmax, ok);
         if (!ok) break;
-        const float top = fmaxf(fmaxf(__bfloat162float(x[threadIdx.x]), __bfloat162float(x[threadIdx.x ^ 64])),
-                                fmaxf(__bfloat162float(x[threadIdx.x ^ 128]), __bfloat162float(x[threadIdx.x ^ 192]))) *
-                          a.scale_log2;
+        const float top =
+            fmaxf(fmaxf(x[threadIdx.x], x[threadIdx.x ^ 64]), fmaxf(x[threadIdx.x ^ 128], x[threadIdx.x ^ 192])) *
+            a.scale_log2;
         const bool move = top > m_ref + kDcRescaleLog2 || m_ref == -INFINITY;
         float f = 1.0f;
         if (move) {

@@ -40,17 +40,17 @@ constexpr int kPfSlots = 8;
 constexpr int kSlotBytes = 16384;
 constexpr int kQSubBytes = 3 * 16384;    // a subtile of Q: three [128 rows][64] chunks
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kPolyEvery = 4;  // every second pair of exponentials by polynomial: the exponential units alone take
-                               // 1024 clocks per subtile and tile of a chain of 4400
+constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial, beside the exponential units' three:
+                               // 16384 tokens of 128 heads 2690 us without, 2330 us with
 
 struct PfSmem {
   static constexpr int kRing = 2 * kQSubBytes;
-  static constexpr int kX = kRing + kPfSlots * kSlotBytes;  // the row's threads' maxima (bf16) or sums
-  static constexpr int kBars = kX + 1024;
+  static constexpr int kX = kRing + kPfSlots * kSlotBytes;  // the rows' threads' maxima or sums
+  static constexpr int kBars = kX + 2 * kPfSoftmax * 4;
   // q, full[8], empty[8], s_full[2], p_full[2], o_full[2], v_ok[2], mma_done
   static constexpr int kNumBars = 1 + 2 * kPfSlots + 9;
   static constexpr int kMisc = kBars + kNumBars * 8;
-  static constexpr int kBytes = kMisc + 64 + 1024;
+  static constexpr int kBytes = kMisc + 64;
 };
 
 struct PfArgs {
@@ -150,8 +150,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                       const __grid_constant__ CUtensorMap map_kr, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ PfArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // the swizzled tiles need 1024 bytes, and there is no room to round a base up
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) record_status(a.status, MOE_ERR_UNSUPPORTED);
+    return;
+  }
   uint8_t* ring = smem + PfSmem::kRing;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PfSmem::kBars);
   uint64_t* q_full = bars;
@@ -438,8 +442,8 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int n_t = n_tiles[sub];
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // 32 lanes per warp
     const uint32_t t_s = lane_base + sub * 128, t_o = lane_base + 256 + sub * 128 + half * 64;
-    __nv_bfloat16* x_max = reinterpret_cast<__nv_bfloat16*>(smem + PfSmem::kX) + sub * kPfSoftmax;
-    float* x_sum = reinterpret_cast<float*>(smem + PfSmem::kX) + sub * kPfTile;
+    float* x_max = reinterpret_cast<float*>(smem + PfSmem::kX) + sub * kPfSoftmax;
+    float* x_sum = x_max;
     const int x_me = half * kPfTile + r;
     float m_ref = -INFINITY, l = 0.f;  // in log2 units of the scaled scores
     bool ok = true;
@@ -471,12 +475,12 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
         for (int x = 0; x < 32; x += 2)
           mx[(x >> 1) & 3] = fmaxf(fmaxf(mx[(x >> 1) & 3], __uint_as_float(raw[c][x])), __uint_as_float(raw[c][x + 1]));
-      // Any common reference near the row's maximum will do: its two threads exchange theirs rounded up to bf16.
-      // The place is free: this tile's scores follow the P that every thread gave after it had read the last ones.
-      x_max[x_me] = __float2bfloat16_ru(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      // The row's two threads exchange their maxima. The place is free: this tile's scores follow the P that
+      // every thread gave after it had read the last ones.
+      x_max[x_me] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       ok = named_bar_and(1 + sub, kPfSoftmax, ok);
       if (!ok) break;
-      const float top = fmaxf(__bfloat162float(x_max[r]), __bfloat162float(x_max[kPfTile + r])) * a.scale_log2;
+      const float top = fmaxf(x_max[r], x_max[kPfTile + r]) * a.scale_log2;
       const bool move = top > m_ref + kRescaleLog2 || m_ref == -INFINITY;
       float f = 1.0f;
       if (move) {
