@@ -146,7 +146,8 @@ def latent_attention_decode(q, cache, block_table, cache_lens, scale, *, out=Non
     if lens.shape[0] != B:
         raise ValueError(f"{name}: cache_lens must have {B} values")
     table = _table(name, block_table, B)
-    q = q.contiguous()
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     shape = (B, n_q, heads, LATENT_DIM)
     if out is None:
         out = torch.empty(shape, dtype=want, device=dev)

@@ -541,8 +541,9 @@ def moe_decode(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, 
     hidden_states [M, K] (bf16 or fp16, M <= ``moe_decode_max_tokens(topk)``), gating_output
     [M, E]; w1 [E, 2N, K] and w2 [E, K, N] in the dtype of hidden_states, or e4m3 with fp32
     ``w1_scale`` / ``w2_scale`` per 128 x 128 block (``quantize_weights_fp8``). With e4m3 weights
-    the tokens and SiLU*mul rows keep their 16 bits (``fused_moe_fp8`` quantises them). Routing
-    as ``grouped_topk``. Returns [M, K] in the dtype of hidden_states.
+    the tokens and SiLU*mul rows are used in 16 bits (``fused_moe_fp8`` quantises them to e4m3): fp16 as
+    it is, bf16 as fp16 under a power of two per row, exact for values above 2^-28 of the
+    row's largest. Routing as ``grouped_topk``. Returns [M, K] in the dtype of hidden_states.
     """
     name = "moe_decode"
     if scoring_func == "softmax":
@@ -585,7 +586,7 @@ def moe_decode(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, 
                          "use moe_layer or grouped_topk with fused_moe_fp8")
     x = hidden_states
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.contiguous()
+        x = x.clone(memory_format=torch.contiguous_format)
     g = gating_output.to(torch.float32).contiguous()
     bias = None
     if e_score_correction_bias is not None:
