@@ -27,7 +27,11 @@
 // the CTA's rows are computed again by the softmax warps, key by key over visible keys only.
 //
 // What bounds it: per 128 keys and CTA the MMAs take 2560 clocks, the exponentials 2048 of the
-// 4-per-clock units of each SM quarter, so the two have to overlap all the time.
+// 4-per-clock units of each SM quarter, so the two have to overlap all the time, and every fourth pair
+// of exponentials is taken off those units by a polynomial. What is left is the chain softmax, PV, QK of each
+// subtile, and power: 128 heads of one causal prompt of 7993 tokens take 2330-2740 us (955-1124
+// TFLOP/s by the box, 0.58-0.68 of the burst bf16 rate), ragged short prompts 58 us, where a CTA's start and its
+// few tiles count.
 #include "latent.h"
 
 namespace moe {
@@ -41,14 +45,14 @@ constexpr int kSlotBytes = 16384;
 constexpr int kQSubBytes = 3 * 16384;    // a subtile of Q: three [128 rows][64] chunks
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial, beside the exponential units' three:
-                               // 16384 tokens of 128 heads 2690 us without, 2330 us with
+                               // 7993 tokens of 128 heads 2690 us without, 2330 us with
 
 struct PfSmem {
   static constexpr int kRing = 2 * kQSubBytes;
   static constexpr int kX = kRing + kPfSlots * kSlotBytes;  // the rows' threads' maxima or sums
   static constexpr int kBars = kX + 2 * kPfSoftmax * 4;
-  // q, full[8], empty[8], s_full[2], p_full[2], o_full[2], v_ok[2], mma_done
-  static constexpr int kNumBars = 1 + 2 * kPfSlots + 9;
+  // q, full[8], empty[8], s_full[2], p_full[2], o_full[2], v_ok[2], v_raw[2], mma_done
+  static constexpr int kNumBars = 1 + 2 * kPfSlots + 11;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kBytes = kMisc + 64;
 };
@@ -165,7 +169,8 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* v_ok = o_full + 2;
-  uint64_t* mma_done = v_ok + 2;
+  uint64_t* v_raw = v_ok + 2;
+  uint64_t* mma_done = v_raw + 2;
   int* misc = reinterpret_cast<int*>(smem + PfSmem::kMisc);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc);
   volatile int* s_abort = misc + 1;
@@ -207,7 +212,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   if (threadIdx.x == 32) {
     mbar_init(q_full, 1);
     for (int s = 0; s < kPfSlots; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kPfSoftmax); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kPfSoftmax); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); mbar_init(&v_raw[i], 2); }
     mbar_init(mma_done, 1);
     *s_abort = 0;
     *s_bad = 0;
@@ -275,7 +280,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
     __syncwarp();
     int slot = 0;
-    uint32_t phase = 0, issued = 0, issued_parity = 0;
+    uint32_t phase = 0, issued = 0, issued_parity = 0, raw_issued = 0, raw_parity = 0;
     bool ok = true;
     for (int j = 0; j < n_max && ok; ++j) {
       const int kt = (int)k_lo + j * kPfTile;
@@ -285,13 +290,25 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           ok = mbar_wait_warp(&empty[slot], phase ^ 1, a.status, s_abort);
           if (ok) {
             uint8_t* dst = ring + slot * kSlotBytes;
+            // V that warps 18-19 look at arrives at a barrier of its own, which they see in every phase; its slot
+            // is passed on at once and the MMAs wait for v_ok. (Had they waited for the slots' barriers, of
+            // which they see V's phases only, a K copy that lands after the V behind it would leave the next phase's
+            // parity looking complete.)
+            const bool look = c >= 3 && j >= sure;
+            const int n = (j - sure) & 1;
             if (one) {
-              mbar_arrive_expect_tx(&full[slot], kSlotBytes);
-              if (c < 2) tma_load_3d(&map_kv, &full[slot], dst, c * 64, kt, h);
-              else if (c == 2) tma_load_2d(&map_kr, &full[slot], dst, 0, kt);
-              else tma_load_4d(&map_v, &full[slot], dst, 0, kt + (c - 3) * 64, 2, h);
+              uint64_t* bar = look ? &v_raw[n] : &full[slot];
+              mbar_arrive_expect_tx(bar, kSlotBytes);
+              if (look) mbar_arrive(&full[slot]);
+              if (c < 2) tma_load_3d(&map_kv, bar, dst, c * 64, kt, h);
+              else if (c == 2) tma_load_2d(&map_kr, bar, dst, 0, kt);
+              else tma_load_4d(&map_v, bar, dst, 0, kt + (c - 3) * 64, 2, h);
             }
             __syncwarp();
+            if (look) {
+              raw_issued |= 1u << n;
+              raw_parity = (raw_parity & ~(1u << n)) | ((uint32_t)((j - sure) >> 1 & 1) << n);
+            }
             issued |= 1u << slot;
             issued_parity = (issued_parity & ~(1u << slot)) | (phase << slot);
             if (++slot == kPfSlots) { slot = 0; phase ^= 1; }
@@ -303,6 +320,8 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       mbar_wait_warp(q_full, 0, nullptr, nullptr);
       for (int s = 0; s < kPfSlots; ++s)
         if ((issued >> s) & 1u) mbar_wait_warp(&full[s], (issued_parity >> s) & 1u, nullptr, nullptr);
+      for (int n = 0; n < 2; ++n)
+        if ((raw_issued >> n) & 1u) mbar_wait_warp(&v_raw[n], (raw_parity >> n) & 1u, nullptr, nullptr);
     }
   } else if (warp == 17) {
     // ------------------------------------------------ MMA issuer: the warp converged, one lane issues
@@ -345,7 +364,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (s >= kPfSlots) { s -= kPfSlots; ph ^= 1; }
     };
     // Everything that PV of a subtile and its next QK need is waited for at once (a wait costs about 125 clocks
-    // when all is there, and a subtile's softmax, PV and QK are one chain): lanes 0-1 V, 2 its check, 3 P, 4-6 K.
+    // when all is there, and a subtile's softmax, PV and QK are one chain): lanes 0-1 V, 2 its check where there is one, 3 P, 4-6 K.
     // A wait that gave up ends the loop at the next tile; until then the MMAs run on what is there.
     auto wait_all = [&](int j, int i, bool pv, bool qk) {
       uint64_t* bar = nullptr;
@@ -353,9 +372,9 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (pv && lane < 2) {
         bar = &full[at(vslot + lane)];
         ph = vslot + lane >= kPfSlots ? vphase ^ 1 : vphase;
-      } else if (pv && lane == 2) {
-        bar = &v_ok[j & 1];
-        ph = (j >> 1) & 1;
+      } else if (pv && lane == 2 && j >= sure) {
+        bar = &v_ok[(j - sure) & 1];
+        ph = ((j - sure) >> 1) & 1;
       } else if (pv && lane == 3) {
         bar = &p_full[i];
         ph = j & 1;
@@ -395,17 +414,14 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     mbar_wait_warp(mma_done, 0, nullptr, nullptr);
   } else if (warp >= 18) {
     // ------------------------------------------------ V where a row may not see a key
-    // They pass every tile on (v_ok, two in turn: the ring holds no more than two tiles' V), so
-    // they see each phase of the ring's barriers.
+    // Two such tiles in turn: the ring holds no more than two tiles' V.
     const int vt = threadIdx.x - (2 * kPfSoftmax + 64);  // 0 .. 63: a key row of each half
-    bool ok = true;
-    for (int j = 0; j < n_max && ok; ++j) {
+    for (int j = sure; j < n_max; ++j) {
+      if (!mbar_wait(&v_raw[(j - sure) & 1], ((j - sure) >> 1) & 1, a.status, s_abort)) break;
       bool wrote = false;
 #pragma unroll 1
       for (int c = 3; c < 5; ++c) {
         const int idx = 5 * j + c;
-        if (!mbar_wait(&full[idx % kPfSlots], (uint32_t)(idx / kPfSlots) & 1u, a.status, s_abort)) { ok = false; break; }
-        if (j < sure) continue;
         uint8_t* base = ring + (idx % kPfSlots) * kSlotBytes + vt * 128;
         const bool past = j * kPfTile + (c - 3) * 64 + vt >= nk;
         uint32_t worst = 0;
@@ -431,7 +447,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         wrote |= past;
       }
       if (wrote) fence_proxy_async_smem();
-      if (ok) mbar_arrive(&v_ok[j & 1]);
+      mbar_arrive(&v_ok[(j - sure) & 1]);
     }
   } else {
     // ------------------------------------------------ softmax, two threads per row
