@@ -509,7 +509,8 @@ MOE_API int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int
  * A whole MoE layer for a few tokens in two kernels: the routing of moe_grouped_topk on
  * gating_output, then sum over the chosen experts of weight * W2 (silu(W1g x) * W1u x), every
  * chosen expert's weights read once. Weights in the tokens' type, or with weight_e4m3 in e4m3
- * with fp32 scales per 128 x 128 block (moe_quantize_blocks_fp8); the tokens keep 16 bits.
+ * with fp32 scales per 128 x 128 block (moe_quantize_blocks_fp8); tokens and activated rows are then
+ * used as fp16, bf16 ones under a power of two per row (exact above 2^-28 of the row's largest).
  * num_tokens <= moe_few_max_tokens(topk) (32, less when topk > 16). ld_hidden: row pitch of
  * hidden_states in elements, a multiple of 8. A token whose logits give no order (NaN) gets NaN.
  */
