@@ -30,7 +30,7 @@
 // 4-per-clock units of each SM quarter, so the two have to overlap all the time, and every fourth pair
 // of exponentials is taken off those units by a polynomial. What is left is the chain softmax, PV, QK of each
 // subtile, and power: 128 heads of one causal prompt of 7993 tokens take 2330-2740 us (955-1124
-// TFLOP/s by the box, 0.58-0.68 of the burst bf16 rate), ragged short prompts 58 us, where a CTA's start and its
+// TFLOP/s by the box, 0.58-0.68 of the burst bf16 rate), ragged prompts of up to 1777 tokens 55 us, where a CTA's start and its
 // few tiles count.
 #include "latent.h"
 

@@ -29,6 +29,9 @@
 // few_down: one CTA per 16 rows of the output; its warps take consecutive runs of the (chunk, k
 //           block) list, add weight * product into their own shared rows in fp32, and the rows are
 //           summed in warp order.
+// Measured, of the bytes of the hit experts at HBM's 6.55 TB/s: e4m3, E 256, K 7168, N 2048: one token 90 us
+// (0.59; the conversions, and about 5 us of routing before the first load), 11 tokens 710-740 us (0.69-0.71); bf16, E 8, K 4096,
+// N 14336, 6 tokens 392-430 us (0.82-0.90).
 // Both give the same bits on every run. Sums are fp32; a_p is rounded once to the tokens' type (the
 // layer's other paths do the same).
 #include "common.cuh"
@@ -558,6 +561,8 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
   FewTables* tab = static_cast<FewTables*>(ws);
   T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(ws) + few_tables_bytes());
   const size_t rows = (size_t)M * (size_t)(K + 8) * 2;
+  // bf16 tokens become fp16 once per CTA where they fit (e4m3 layer of K 7168: one token 94 -> 90 us, 11
+  // tokens 740 -> 708 us); more tokens are converted as they are read
   const bool staged = F8 && ElemTraits<T>::kFmt == 1 && sizeof(UpShared) + rows <= kUpMaxSmem;
   const size_t smem = sizeof(UpShared) + (staged ? rows : 0);
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(few_up_kernel<T, F8>), (int)smem);
@@ -569,7 +574,9 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
   few_up_kernel<T, F8><<<num_sms(), 32 * kUpWarps, smem, st>>>(
       static_cast<const T*>(x), ld_x, rt, static_cast<const uint8_t*>(w1), w1s, M, E, K, N, staged, act, tab);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
-  // about 16 warps per SM over all CTAs, so that few rows of output still ask for enough bytes at once
+  // about 16 warps per SM over all CTAs, so that few rows of output still ask for enough bytes at once. Measured
+  // with 4, 8 and 16 warps, us: e4m3, K 7168, N 2048, 1 token 31, 34, 40, 11 tokens 245, 254, 269; bf16, K 4096,
+  // N 14336, 6 tokens 225, 147, 155; bf16, K 2048, N 1408, 4 tokens of 6 experts 72, 41, 29, 1 token 21, 14, 11
   const int ctas = K / 16;
   const int warps = ctas * 6 > num_sms() * 16 ? 4 : ctas * 12 > num_sms() * 16 ? 8 : 16;
   auto kern = warps == 4 ? few_down_kernel<T, F8, 4> : warps == 8 ? few_down_kernel<T, F8, 8> : few_down_kernel<T, F8, 16>;
