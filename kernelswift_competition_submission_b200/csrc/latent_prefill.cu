@@ -24,7 +24,9 @@
 // Masked places: a score is replaced before the maximum is taken, so keys may hold anything.
 // V meets P = 0 in the MMA, and 0 * NaN is NaN, so warps 18-19 zero the V rows past the request's
 // end, and look for non-finite values in tiles that some row sees only in part; if there is one,
-// the CTA's rows are computed again by the softmax warps, key by key over visible keys only.
+// the rows of the subtiles that walk the tile are computed again by the softmax warps, key by key over visible
+// keys only. A subtile asks for its own tiles alone, and after their look, so its answer does not depend on when
+// the other subtile's next V lands.
 //
 // What bounds it: per 128 keys and CTA the MMAs take 2560 clocks, the exponentials 2048 of the
 // 4-per-clock units of each SM quarter, so the two have to overlap all the time, and every fourth pair
@@ -174,8 +176,9 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   int* misc = reinterpret_cast<int*>(smem + PfSmem::kMisc);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(misc);
   volatile int* s_abort = misc + 1;
-  volatile int* s_bad = misc + 2;
+  volatile int* s_bad = misc + 2;  // [2]: a V tile that the subtile walks holds a non-finite value
   int* s_unit = misc + 4;  // request, tile
+  volatile int* s_look = misc + 6;  // [2]: a subtile's tiles from the first that is looked at, less one
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x / a.units;
@@ -215,7 +218,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], kPfSoftmax); mbar_init(&o_full[i], 1); mbar_init(&v_ok[i], 64); mbar_init(&v_raw[i], 2); }
     mbar_init(mma_done, 1);
     *s_abort = 0;
-    *s_bad = 0;
+    s_bad[0] = s_bad[1] = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -246,6 +249,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int sure = min(nk, a.causal ? max(0, nk - nq + 1 + row0) : nk) / kPfTile;  // tiles all rows see whole
 
   if (n_max > 0) {
+    if (threadIdx.x < 2) s_look[threadIdx.x] = (threadIdx.x ? n_tiles[1] : n_tiles[0]) - 1 - sure;
     if (warp == 17) { tmem_alloc(s_tmem, 512); tmem_relinquish(); }
     tc_fence_before();
   }
@@ -443,7 +447,10 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
           }
         }
-        if (worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) *s_bad = 1;
+        if (worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) {
+          if (j < n_tiles[0]) s_bad[0] = 1;
+          if (j < n_tiles[1]) s_bad[1] = 1;
+        }
         wrote |= past;
       }
       if (wrote) fence_proxy_async_smem();
@@ -455,7 +462,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int r = (warp & 3) * 32 + lane;                // row of the subtile
     const int i_row = row0 + sub * kPfTile + r;          // row of the request
     const int limit = seen(i_row);
-    const int n_t = n_tiles[sub];
+    const int n_t = sub ? n_tiles[1] : n_tiles[0];
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);  // 32 lanes per warp
     const uint32_t t_s = lane_base + sub * 128, t_o = lane_base + 256 + sub * 128 + half * 64;
     float* x_max = reinterpret_cast<float*>(smem + PfSmem::kX) + sub * kPfSoftmax;
@@ -544,6 +551,10 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       mbar_arrive(&p_full[sub]);
     }
     if (n_t > 0) ok = mbar_wait(&o_full[sub], 0, a.status, s_abort) && ok;
+    // The look at the subtile's last tile, and with it at all before: its s_bad no longer changes. (The other
+    // subtile walks one tile more at most, on the other barrier, so this phase is the barrier's latest.)
+    const int looked = s_look[sub];
+    if (looked >= 0) ok = mbar_wait(&v_ok[looked & 1], (looked >> 1) & 1, a.status, s_abort) && ok;
     tc_fence_after();
     ok = named_bar_and(1 + sub, kPfSoftmax, ok);  // the last maxima are read
     if (half == 1) x_sum[r] = l;
@@ -556,7 +567,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     l = x_sum[r];
     const bool live = i_row < nq;
     const int64_t row = (q_lo + i_row) * a.heads + h;
-    if (*s_bad) {
+    if (s_bad[sub]) {
       if (ok)
         for (int rr = warp & 7; rr < kPfTile; rr += kPfSoftmax / 32) {
           const int i = row0 + sub * kPfTile + rr;
