@@ -468,9 +468,10 @@ MOE_API int moe_latent_cache_write(int dtype, const void* latent, int64_t ld_lat
                                    void* cache, int64_t num_pages, int page_size, int* status, void* stream);
 
 /* Reads contexts back as contiguous rows: row cu_lens[b] + j of latent [total, 512] and k_rope
- * [total, 64] is position j of request b, in the cache's type (bf16 from e4m3 pages). Rows past
- * cu_lens[num_seqs] are zeros; positions whose page is outside the cache or past the table read
- * as NaN and are recorded in `status`. block_table int32 [num_seqs, table_width], pitch ld_table. */
+ * [total, 64] is position j of request b, in the cache's type (bf16 from e4m3 pages). cu_lens
+ * ascends; rows before cu_lens[0] and past cu_lens[num_seqs] are zeros; positions whose page is
+ * outside the cache or past the table read as NaN and are recorded in `status`. block_table int32
+ * [num_seqs, table_width], pitch ld_table. */
 MOE_API int moe_latent_cache_read(int cache_fmt, const void* cache, int64_t num_pages, int page_size,
                                   const int32_t* block_table, int64_t ld_table, int table_width,
                                   const int32_t* cu_lens, int num_seqs, int64_t total, void* latent, void* k_rope,

@@ -103,9 +103,9 @@ def latent_cache_write(cache: torch.Tensor, latent: torch.Tensor, k_rope: torch.
 def latent_cache_read(cache: torch.Tensor, block_table: torch.Tensor, cu_lens: torch.Tensor, total: int):
     """The first cu_lens[b + 1] - cu_lens[b] positions of every request as contiguous rows:
     (latent [total, 512], k_rope [total, 64]) in the cache's dtype, bf16 from an e4m3 cache
-    (codes times power-of-two scales: exact). block_table [B, pages], cu_lens [B + 1] ascending from
-    0 (int32, on the device), total = cu_lens[B] as the caller knows it on the host. Positions
-    without a valid page read as NaN and are reported by ``check_device_status``."""
+    (codes times power-of-two scales: exact). block_table [B, pages], cu_lens [B + 1] ascending
+    (int32, on the device), total = cu_lens[B] as the caller knows it on the host. Rows before cu_lens[0] and
+    past cu_lens[B] are zeros. Positions without a valid page read as NaN and are reported by ``check_device_status``."""
     name = "latent_cache_read"
     dev = _require_cuda(name, cache, block_table, cu_lens)
     fmt = _cache_fmt(name, cache)

@@ -109,7 +109,7 @@ latent_cache_write_kernel(const T* __restrict__ latent, int64_t ld_latent, bool 
 }
 
 // Row i of the output is position i - cu_lens[b] of request b, cu_lens[b] <= i < cu_lens[b + 1];
-// rows past cu_lens[num_seqs] are zeros. A table entry outside the cache, or a position past
+// rows before cu_lens[0] and past cu_lens[num_seqs] are zeros. A table entry outside the cache, or a position past
 // the table, records MOE_ERR_INVALID_ARG and reads as NaN.
 template <bool E4M3>
 __global__ void __launch_bounds__(kCacheThreads)
@@ -127,7 +127,7 @@ latent_cache_read_kernel(const uint8_t* __restrict__ cache, int64_t num_pages, i
   }
   uint4* dst = reinterpret_cast<uint4*>(latent + i * kLatDim) + lane * 2;
   uint32_t* rdst = reinterpret_cast<uint32_t*>(k_rope + i * kRopeDim) + lane;
-  if (lo >= num_seqs) {
+  if (lo >= num_seqs || (int64_t)__ldg(cu_lens + lo) > i) {  // no request's row
     dst[0] = dst[1] = make_uint4(0u, 0u, 0u, 0u);
     *rdst = 0u;
     return;
