@@ -497,8 +497,8 @@ MOE_API int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int q_
  * output), k_rope [total_k, 64] shared by the heads; strides in elements (multiples of 8), last
  * dimension contiguous. Request b has query rows cu_q[b] .. cu_q[b + 1] and keys cu_k[b] ..
  * cu_k[b + 1]; with `causal` its last query sees all its keys, the one before one key less, and
- * so on. out [total_q, heads, 128], lse (optional) fp32 [total_q, heads]; rows that see nothing,
- * and rows past cu_q[num_seqs], give zeros and -inf.
+ * so on. cu_q and cu_k ascend. out [total_q, heads, 128], lse (optional) fp32 [total_q, heads];
+ * rows that see nothing, and rows before cu_q[0] or past cu_q[num_seqs], give zeros and -inf.
  */
 MOE_API int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
                                int64_t kv_stride_t, int64_t kv_stride_h, const void* k_rope, int64_t kr_stride_t,

@@ -186,11 +186,11 @@ def latent_attention_prefill(q, kv, k_rope, cu_q, cu_k, scale, *, causal=True, o
 
     q [Tq, heads, 192] (128 without position, 64 rotary), kv [Tk, heads, 256] (128 key values
     without position, then 128 value values: the up-projection's output), k_rope [Tk, 64] shared by
-    all heads; bf16 or fp16, views with strides are read in place. cu_q, cu_k int32 [B + 1]: request
+    all heads; bf16 or fp16, views with strides are read in place. cu_q, cu_k int32 [B + 1], ascending: request
     b's queries and keys. ``causal``: the last query sees all keys, the one before it one less, and
     so on (queries are the last tokens of their context). Returns out [Tq, heads, 128] and with
     ``return_lse`` also the natural log-sum-exp fp32 [Tq, heads], by which pieces of a context can be
-    joined; a row that sees nothing gives zeros and -inf."""
+    joined; a row that sees nothing, or that belongs to no request, gives zeros and -inf."""
     name = "latent_attention_prefill"
     dev = _require_cuda(name, q, kv, k_rope, cu_q, cu_k)
     dt = q.dtype

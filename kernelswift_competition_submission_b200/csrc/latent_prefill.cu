@@ -184,8 +184,9 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int h = blockIdx.x / a.units;
   const int unit = a.units - 1 - (blockIdx.x - h * a.units);
 
-  // which request and tile: prefix of ceil(rows / 256); the rows past cu_q[num_seqs] are one more
-  // request without keys
+  // which request and tile: prefix of ceil(rows / 256); the rows before cu_q[0] and those past
+  // cu_q[num_seqs] are together one more request without keys
+  const int64_t lead = min((int64_t)max(__ldg(a.cu_q), 0), a.tq);
   if (warp == 0) {
     int base = 0, found = -1, tile = 0;
     for (int b0 = 0; b0 <= a.num_seqs && found < 0; b0 += 32) {
@@ -193,7 +194,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       int n = 0;
       if (b <= a.num_seqs) {
         const int64_t lo = min((int64_t)max(__ldg(a.cu_q + b), 0), a.tq);
-        const int64_t hi = b < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + b + 1), 0), a.tq) : a.tq;
+        const int64_t hi = b < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + b + 1), 0), a.tq) : a.tq + lead;
         n = hi > lo ? (int)((hi - lo + 255) / 256) : 0;
       }
       int inc = n;
@@ -225,7 +226,7 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int req = s_unit[0];
   if (req < 0) return;  // past the last unit: nothing allocated, nothing in flight
   const int64_t q_lo = min((int64_t)max(__ldg(a.cu_q + req), 0), a.tq);
-  const int64_t q_hi = req < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + req + 1), 0), a.tq) : a.tq;
+  const int64_t q_hi = req < a.num_seqs ? min((int64_t)max(__ldg(a.cu_q + req + 1), 0), a.tq) : a.tq + lead;
   const int nq = (int)(q_hi - q_lo);
   int64_t k_lo = 0;
   int nk = 0;
@@ -258,7 +259,8 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (warp < 8) {  // 256 rows
       const int i = row0 + threadIdx.x;
       if (i < nq) {
-        const int64_t row = (q_lo + i) * a.heads + h;
+        // past the last request the rows go on at 0
+        const int64_t row = (q_lo + i < a.tq ? q_lo + i : q_lo + i - a.tq) * a.heads + h;
         uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * kNopeDim);
 #pragma unroll
         for (int c = 0; c < 16; ++c) o[c] = make_uint4(0u, 0u, 0u, 0u);
