@@ -78,7 +78,7 @@ def latent_cache_write(cache: torch.Tensor, latent: torch.Tensor, k_rope: torch.
     ``slots`` [n] = page * page_size + offset; negative slots are skipped. 16-bit caches take their
     own dtype; an e4m3 cache takes bf16 and quantises each 128 latent values with the power-of-two
     scale of ``quantize_rows_fp8`` (non-finite values are kept as NaN and leave their block's scale
-    alone). Slots past the cache are skipped and reported by ``check_device_status``."""
+    alone; finite ones read back finite: those that would round to 2^128 take 15/16 of it). Slots past the cache are skipped and reported by ``check_device_status``."""
     name = "latent_cache_write"
     dev = _require_cuda(name, cache, latent, k_rope, slots)
     fmt = _cache_fmt(name, cache)

@@ -2,7 +2,9 @@
 // as contiguous rows for the expanded form of latent attention. Layout: latent.h.
 //
 //   write: s_b = 2^ceil(log2(amax_b / 448)) over each 128 latent values (1 for a zero block),
-//          code = e4m3(x / s_b), nearest even: x / s_b is exact, so one rounding per value.
+//          code = e4m3(x / s_b), nearest even: x / s_b is exact, so one rounding per value. Values
+//          that would round up to 256 * 2^120 = 2^128, beyond fp32 and bf16 alike, take 240 * 2^120:
+//          a finite value reads back finite (a larger s_b would not help, 255 has no nearer code).
 //          amax_b counts finite values only; an infinity or NaN is stored as e4m3 NaN and
 //          reads back as NaN without touching its block's other values. Rotary keys keep
 //          their 16 bits (their products carry the position and are 1/9 of the row).
@@ -22,6 +24,7 @@ namespace moe {
 namespace {
 
 constexpr int kCacheThreads = 256;
+constexpr float kLargestBack = 0x1.Ep127f;  // 240 * 2^120, see write
 
 template <typename T>
 __device__ __forceinline__ void load16(const T* p, bool vec, uint32_t (&w)[8]) {
@@ -93,7 +96,8 @@ latent_cache_write_kernel(const T* __restrict__ latent, int64_t ld_latent, bool 
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const uint32_t c = fabsf(v[j]) < INFINITY
-                             ? (uint32_t)__nv_cvt_float_to_fp8(v[j] / sc, __NV_SATFINITE, __NV_E4M3)
+                             ? (uint32_t)__nv_cvt_float_to_fp8(fminf(fmaxf(v[j], -kLargestBack), kLargestBack) / sc,
+                                                               __NV_SATFINITE, __NV_E4M3)
                              : 0x7Fu;
       q[j >> 2] |= c << (8 * (j & 3));
     }
