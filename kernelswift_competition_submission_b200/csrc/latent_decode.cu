@@ -631,16 +631,17 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const uint32_t f = min(scale[u] + 120u, 254u) * 0x00800080u, f2 = (scale[u] - 7u) * 0x00800080u;
           widen8(q0, f, scale[u] > 134u, f2, nan, v0);
           widen8(q1, f, scale[u] > 134u, f2, nan, v1);
-          if (nan & 0x80808080u) {
+          // above 246 a code may widen to infinity (448 x 2^(e - 127) from 2^128 up)
+          if ((nan & 0x80808080u) != 0u || scale[u] > 246u) {
             nan8(q0, v0);
             nan8(q1, v1);
-            bad |= key >= sure;
+            bad |= key >= sure && key < sg.len;
           }
           __syncwarp();
           *reinterpret_cast<uint4*>(row + u * (kStride * 128) + o0) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
           *reinterpret_cast<uint4*>(row + u * (kStride * 128) + o1) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
         }
-        // values that some query may not see must not be NaN under its P = 0
+        // values that some query may not see must not be NaN or infinite under its P = 0
         if (for_v && __any_sync(0xffffffffu, bad) && lane < 2) {
           const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
           asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
