@@ -249,6 +249,13 @@ __device__ __forceinline__ void nan8(uint2 q, uint32_t (&o)[4]) {
   }
 }
 
+// Marks a segment in CTA `rank`'s s_bad. The barriers that follow order by CTA scope only, so the mark is released to the
+// cluster here, and acquired once per segment by the softmax warps that read it.
+__device__ __forceinline__ void flag_bad(const int* flag, uint32_t rank, int mark) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(flag, rank)), "r"(mark) : "memory");
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
 latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_c,
@@ -461,10 +468,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           }
         }
       }
-      if (__any_sync(0xffffffffu, worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) && lane < 2) {
-        const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
-      }
+      if (__any_sync(0xffffffffu, worst >= (ElemTraits<T>::kFmt == 1 ? 0x7F80u : 0x7C00u)) && lane < 2)
+        flag_bad(const_cast<const int*>(s_bad) + (seg & 1), (uint32_t)lane, seg + 1);
       fence_proxy_async_smem();
       __syncwarp();
       if (one) {
@@ -642,10 +647,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           *reinterpret_cast<uint4*>(row + u * (kStride * 128) + o1) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
         }
         // values that some query may not see must not be NaN or infinite under its P = 0
-        if (for_v && __any_sync(0xffffffffu, bad) && lane < 2) {
-          const uint32_t dst = mapa_shared(const_cast<int*>(s_bad) + (seg & 1), (uint32_t)lane);
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(seg + 1) : "memory");
-        }
+        if (for_v && __any_sync(0xffffffffu, bad) && lane < 2)
+          flag_bad(const_cast<const int*>(s_bad) + (seg & 1), (uint32_t)lane, seg + 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(full0 + slot * 8);
@@ -790,6 +793,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const bool whole = sg.k0 == 0 && sg.k1 == sg.n;
       const int64_t pslot = 2 * pair + (sg.k0 == 0 ? 1 : 0);
       const bool live = row < a.rows;
+      asm volatile("fence.acq_rel.cluster;" ::: "memory");  // flag_bad of either CTA, ahead of the products in pv_done
       if (s_bad[seg & 1] == seg + 1) {
         tc_fence_before();
         __syncwarp();
