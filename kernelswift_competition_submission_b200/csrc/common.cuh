@@ -57,16 +57,19 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait for the phase with the given parity to complete.
+// Bounded wait for the phase with the given parity to complete. `hold`: two words; while one is set, what is
+// waited for is known to be at work that itself ends, and the limit starts over.
+__device__ __forceinline__ bool wait_held(const volatile int* hold) { return hold && (hold[0] | hold[1]); }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status,
-                                          volatile int* abort_flag) {
+                                          volatile int* abort_flag, const volatile int* hold = nullptr) {
   if (mbar_test(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = globaltimer_ns();
   uint32_t it = 0;
   while (true) {
     if (mbar_test(bar, parity)) return true;
     if ((++it & 63u) == 0) {
       if (abort_flag && *abort_flag) return false;
+      if (wait_held(hold)) t0 = globaltimer_ns();
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
         record_status(status, MOE_ERR_TIMEOUT);
         if (abort_flag) *abort_flag = 1;
@@ -89,14 +92,16 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 // mbar_wait by a whole warp: every lane gets the same answer, and the warp stays converged.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag,
+                                               const volatile int* hold = nullptr) {
   if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = globaltimer_ns();
   uint32_t it = 0;
   while (true) {
     if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
     if ((++it & 63u) == 0) {
       bool stop = abort_flag && *abort_flag;
+      if (wait_held(hold)) t0 = globaltimer_ns();
       if (!stop && globaltimer_ns() - t0 > kWaitLimitNs) {
         record_status(status, MOE_ERR_TIMEOUT);
         if (abort_flag) *abort_flag = 1;
@@ -108,16 +113,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
 }
 // The same for several barriers at once: lane l waits on its own `bar` (nullptr: on none). One wait costs
 // about 125 clocks when everything is there already, during which the warp issues nothing.
-__device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag) {
+__device__ __forceinline__ bool mbar_wait_lanes(uint64_t* bar, uint32_t parity, int* status, volatile int* abort_flag,
+                                                const volatile int* hold = nullptr) {
   bool done = bar == nullptr || mbar_test(bar, parity);
   if (__all_sync(0xffffffffu, done)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = globaltimer_ns();
   uint32_t it = 0;
   while (true) {
     done = done || mbar_test(bar, parity);
     if (__all_sync(0xffffffffu, done)) return true;
     if ((++it & 63u) == 0) {
       bool stop = abort_flag && *abort_flag;
+      if (wait_held(hold)) t0 = globaltimer_ns();
       if (!stop && globaltimer_ns() - t0 > kWaitLimitNs) {
         record_status(status, MOE_ERR_TIMEOUT);
         if (abort_flag) *abort_flag = 1;

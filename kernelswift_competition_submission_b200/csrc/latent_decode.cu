@@ -26,7 +26,7 @@
 // Masked places: scores are replaced before the maximum. V meets P = 0 in the MMA and 0 * NaN is
 // NaN, so in tiles that some row does not see whole the producer zeroes V past the length and looks
 // for non-finite values before the draft tokens; if there is one, the rows are computed again key by
-// key over visible keys.
+// key over visible keys, while the pair's other waits hold their limit (s_hold).
 //
 // Measured on the device, 74 requests of 2560 tokens: 16-bit pages 56 us with 128 heads (935 TFLOP/s, 0.57 of
 // the burst bf16 rate) and 55 us with 16 (3.95 TB/s, 0.60 of HBM); e4m3 pages 111 us with either.
@@ -255,6 +255,10 @@ __device__ __forceinline__ void flag_bad(const int* flag, uint32_t rank, int mar
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(flag, rank)), "r"(mark) : "memory");
   asm volatile("fence.acq_rel.cluster;" ::: "memory");
 }
+// Sets a word of CTA `rank`'s s_hold; it orders nothing.
+__device__ __forceinline__ void set_hold(const int* word, uint32_t rank, int value) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(mapa_shared(word, rank)), "r"(value) : "memory");
+}
 
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(E4M3 ? kDcThreads8 : kDcThreads, 1)
@@ -291,6 +295,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   volatile int* s_bad = misc + 2;        // [2]: segment number + 1 whose V holds a non-finite value
   volatile int* s_badpage = misc + 4;
   int* s_plan = misc + 6;                // request, offset (2 words), tiles (2 words)
+  volatile int* s_hold = misc + 12;      // [2]: a CTA of the pair computes rows key by key
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -342,6 +347,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     *s_abort = 0;
     s_bad[0] = s_bad[1] = 0;
     *s_badpage = 0;
+    s_hold[0] = s_hold[1] = 0;
     fence_mbar_init();
   }
   if (warp == 9) { tmem_alloc_pair(s_tmem, 512); tmem_relinquish_pair(); }
@@ -403,7 +409,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, pages, half * 4 + ((i * br) >> 4 & 3));
     };
     auto wait_two = [&](int c) {  // slots c, c + 1 of this warp's four have been read
-      return mbar_wait_lanes(lane < 2 ? &empty[slot0 + c + lane] : nullptr, (g & 1u) ^ 1u, a.status, s_abort);
+      return mbar_wait_lanes(lane < 2 ? &empty[slot0 + c + lane] : nullptr, (g & 1u) ^ 1u, a.status, s_abort, s_hold);
     };
     auto load_k = [&](int pages, int j) {
       int pg[4];
@@ -417,7 +423,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         __syncwarp();
       }
-      if (!mbar_wait_warp(rope_free, (g & 1u) ^ 1u, a.status, s_abort)) return false;
+      if (!mbar_wait_warp(rope_free, (g & 1u) ^ 1u, a.status, s_abort, s_hold)) return false;
       if (one) {
         const int row = br == 64 ? (j * kDcTile + (int)rank * 64) & (a.page_size - 1) : 0;
         if (rank == 0) mbar_arrive_expect_tx(rope_full, 2 * 8192);
@@ -449,7 +455,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       if (!local) return true;
       // some row does not see all of this tile: V came in on this CTA's own barrier; zero the rows past the
       // length, look at the rows some query may not see, then hand the slots over
-      if (!mbar_wait_warp(fix, fix_phase, a.status, s_abort)) return false;
+      if (!mbar_wait_warp(fix, fix_phase, a.status, s_abort, s_hold)) return false;
       fix_phase ^= 1;
       uint32_t worst = 0;
       for (int c = 0; c < 4; ++c) {
@@ -491,7 +497,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
       } else {
         // the query rows of the segment before are no longer read
-        if (seg > 0 && !mbar_wait_warp(q_free, (seg - 1) & 1, a.status, s_abort)) { ok = false; break; }
+        if (seg > 0 && !mbar_wait_warp(q_free, (seg - 1) & 1, a.status, s_abort, s_hold)) { ok = false; break; }
         if (one) {
           if (rank == 0) mbar_arrive_expect_tx(q_full, 2 * 9 * 8192);
           tma_load_4d_pair(&map_q, mapa_shared(q_full, 0), smem, 0, sg.rt * kDcTile + (int)rank * kDcRows, 0, sg.b);
@@ -521,7 +527,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const uint64_t dq0 = smem_desc_sw128(smem), dk0 = smem_desc_sw128(ring), dp0 = smem_desc_sw128(s_p);
       const uint64_t dv0 = smem_desc_mn_sw128(ring + 4 * kDcSlotBytes, 8192), dr0 = smem_desc_sw128(smem + DcSmem::kRope);
       auto wait_for = [&](uint64_t* bar, uint32_t phase) {
-        ok = mbar_wait_warp(bar, phase, a.status, s_abort) && ok;
+        ok = mbar_wait_warp(bar, phase, a.status, s_abort, s_hold) && ok;
         tc_fence_after();
       };
       // S of the run's tile `tile`; last: nothing reads the segment's Q after it
@@ -610,7 +616,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const int half = for_v ? (c & 1) : (int)rank, blk = for_v ? (c & 2) + (int)rank : c;
         uint8_t* base = ring + slot * kDcSlotBytes;
         const int first = j * kDcTile + half * 64;
-        ok = mbar_wait_warp(&raw[slot], g & 1u, a.status, s_abort) && ok;
+        ok = mbar_wait_warp(&raw[slot], g & 1u, a.status, s_abort, s_hold) && ok;
         // scale bytes: TMA writes start on 128 bytes, with pages of 16 keys a page's 64 bytes are that far apart
         uint32_t scale[64 / kStride];
 #pragma unroll
@@ -697,7 +703,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const bool bad_page = *s_badpage == seg + 1;
       for (int j = sg.k0; j < sg.k1; ++j, ++g) {
         // a wait that gave up is carried to the next barrier of the softmax warps, so that all leave together
-        ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort) && ok;
+        ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, a.status, s_abort, s_hold) && ok;
         tc_fence_after();
         uint32_t raw[32];
         tmem_ld32(lane_base + kTmemS + (g & 1) * 64 + quarter * 32, raw);
@@ -755,7 +761,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (j > sg.k0) {  // PV of the tile before: its P is read, its O is written
-          ok = mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort) && ok;
+          ok = mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort, s_hold) && ok;
           tc_fence_after();
           if (__any_sync(0xffffffffu, move && f != 1.0f)) {
             const float w = move ? f : 1.0f;
@@ -781,7 +787,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(p_full, 0));
       }
-      ok = ok && mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort);
+      ok = ok && mbar_wait(pv_done, (g - 1) & 1, a.status, s_abort, s_hold);
       tc_fence_after();
       // ---------------------------------------------- end of the segment
       ok = named_bar_and(1, kDcSoftmax, ok);  // the maxima of the last tile are read
@@ -795,6 +801,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const bool live = row < a.rows;
       asm volatile("fence.acq_rel.cluster;" ::: "memory");  // flag_bad of either CTA, ahead of the products in pv_done
       if (s_bad[seg & 1] == seg + 1) {
+        // rows of a long segment take longer than a wait may: the pair's waits are told
+        if (threadIdx.x < 2) set_hold(const_cast<const int*>(s_hold) + rank, threadIdx.x, 1);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(mapa_shared(o_free, 0));
@@ -820,6 +828,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             if (lane == 0) a.part_ml[o] = make_float2(m * 1.4426950408889634f, ls);
           }
         }
+        named_bar_sync(1, kDcSoftmax);  // all warps' rows
+        if (threadIdx.x < 2) set_hold(const_cast<const int*>(s_hold) + rank, threadIdx.x, 0);
       } else {
         const bool some = l > 0.f || l != l;
         const float inv = some ? 1.0f / l : 0.f;
