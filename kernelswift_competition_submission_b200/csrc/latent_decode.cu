@@ -513,8 +513,12 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
       ++seg;
     }
-    if (!ok && (E4M3 || rank == 0) && g > 0) {  // wait (bounded) for the last copies before the pair may leave
-      for (int c = 0; c < 4; ++c) mbar_wait_warp(E4M3 ? &raw[slot0 + c] : &full[slot0 + c], (g - 1) & 1u, nullptr, nullptr);
+    if (!ok) {
+      // Copies in flight have to land before the pair may leave. The other CTA's are counted on the first one's
+      // barriers, and phases stay open for good where one of the two has stopped, so this warp waits out a time
+      // instead: ten thousand times what a copy takes.
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 10000000ull) __nanosleep(1000);
     }
   } else if (warp == 9) {
     if (rank == 0) {
