@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _DTYPES, _ptr, _require_cuda, _stream, status_word
+from .ops import _DTYPES, _ptr, _require_cuda, _stream, _workspace, status_word
 
 LATENT_DIM = 512
 ROPE_DIM = 64
@@ -156,9 +156,7 @@ def latent_attention_decode(q, cache, block_table, cache_lens, scale, *, out=Non
     lse = torch.empty(B, n_q, heads, dtype=torch.float32, device=dev) if return_lse else None
     lib = _lib.load()
     if B and n_q and heads:
-        need = int(lib.moe_latent_decode_workspace_bytes(B, n_q, heads))
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = _workspace(name, workspace, int(lib.moe_latent_decode_workspace_bytes(B, n_q, heads)), dev)
         _lib.check(
             lib.moe_latent_decode(_DTYPES[want], _ptr(q), B, n_q, heads, fmt, _ptr(cache), cache.shape[0],
                                   cache.shape[1], _ptr(table), table.stride(0), table.shape[1], _ptr(lens),

@@ -51,6 +51,15 @@ def _require_cuda(name: str, *ts: torch.Tensor) -> torch.device:
     return dev
 
 
+def _workspace(name: str, workspace: torch.Tensor | None, need: int, dev: torch.device) -> torch.Tensor:
+    """The caller's workspace when it holds `need` bytes, else a new one; its address goes to kernels as it is."""
+    if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+        raise ValueError(f"{name}: workspace must be a contiguous tensor on {dev}")
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    return workspace
+
+
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 the kernels write MOE_ERR_TIMEOUT into if a bounded wait gives up."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -598,9 +607,7 @@ def moe_decode(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, 
         out = torch.empty(M, K, dtype=dt, device=dev)
     elif tuple(out.shape) != (M, K) or out.dtype != dt or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"{name}: out must be a contiguous {dt} [{M}, {K}] tensor on {dev}")
-    need = int(lib.moe_few_workspace_bytes(M, topk, N))
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+    workspace = _workspace(name, workspace, max(int(lib.moe_few_workspace_bytes(M, topk, N)), 256), dev)
     _lib.check(
         lib.moe_few_tokens(_DTYPES[dt], _ptr(x), x.stride(0), _ptr(g), _ptr(bias), int(f8), _ptr(w1), _ptr(s1),
                            _ptr(w2), _ptr(s2), M, E, topk, int(bool(renormalize)), num_expert_group, topk_group, sf,
