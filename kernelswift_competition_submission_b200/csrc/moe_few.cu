@@ -49,7 +49,7 @@ constexpr int kFewMaxTokens = 32;
 constexpr int kFewMaxPairs = 512;
 constexpr int kFewCols = 8;          // pairs per chunk: the MMA's columns
 constexpr int kUpWarps = 12;
-constexpr size_t kUpMaxSmem = 200 * 1024;
+constexpr size_t kUpMaxSmem = 160 * 1024;  // with the tokens' fp16 copies, see launch_few
 constexpr int kBlkBytes = 128;       // weight bytes of a row per k block
 
 // Written by few_up's first CTA for few_down.
@@ -561,8 +561,9 @@ cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const 
   FewTables* tab = static_cast<FewTables*>(ws);
   T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(ws) + few_tables_bytes());
   const size_t rows = (size_t)M * (size_t)(K + 8) * 2;
-  // bf16 tokens become fp16 once per CTA where they fit (e4m3 layer of K 7168: one token 94 -> 90 us, 11
-  // tokens 740 -> 708 us); more tokens are converted as they are read
+  // A few bf16 tokens become fp16 once per CTA, more of them as they are read. e4m3, E 256, K 7168, N 2048, us, once against
+  // as read: 1 token 99/102, 2 169/174, 4 294/305, 6 425/428, but 8 600/551 and 9 664/612, where the copies leave little
+  // of the SM's memory to L1; so up to 160 KB with the tables, 6 tokens of that width
   const bool staged = F8 && ElemTraits<T>::kFmt == 1 && sizeof(UpShared) + rows <= kUpMaxSmem;
   const size_t smem = sizeof(UpShared) + (staged ? rows : 0);
   cudaError_t err = ensure_smem_limit(reinterpret_cast<const void*>(few_up_kernel<T, F8>), (int)smem);
