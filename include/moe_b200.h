@@ -462,7 +462,8 @@ MOE_API int64_t moe_latent_cache_page_bytes(int cache_fmt, int page_size);
 /* Writes num_tokens rows (latent [n, 512] and k_rope [n, 64] of `dtype`, row pitches in
  * elements, any alignment of the type) to slots[i] = page * page_size + offset; negative slots
  * are skipped, slots past the cache are skipped and recorded in `status`. 16-bit pages take
- * their own dtype, e4m3 pages bf16. Two rows for one slot: one of them is kept. */
+ * their own dtype, e4m3 pages bf16. A slot may be given once per call: of two rows for one, parts of
+ * either may be kept. Finite values stay finite in e4m3 (what would round to 2^128 takes 15/16 of it). */
 MOE_API int moe_latent_cache_write(int dtype, const void* latent, int64_t ld_latent, const void* k_rope,
                                    int64_t ld_rope, const int64_t* slots, int64_t num_tokens, int cache_fmt,
                                    void* cache, int64_t num_pages, int page_size, int* status, void* stream);
@@ -508,8 +509,8 @@ MOE_API int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, int
 
 /*
  * A whole MoE layer for a few tokens in two kernels: the routing of moe_grouped_topk on
- * gating_output, then sum over the chosen experts of weight * W2 (silu(W1g x) * W1u x), every
- * chosen expert's weights read once. Weights in the tokens' type, or with weight_e4m3 in e4m3
+ * gating_output, then sum over the chosen experts of weight * W2 (silu(W1g x) * W1u x), a chosen
+ * expert's weights read once per 8 of its tokens. Weights in the tokens' type, or with weight_e4m3 in e4m3
  * with fp32 scales per 128 x 128 block (moe_quantize_blocks_fp8); tokens and activated rows are then
  * used as fp16, bf16 ones under a power of two per row (exact above 2^-28 of the row's largest).
  * num_tokens <= moe_few_max_tokens(topk) (32, less when topk > 16). ld_hidden: row pitch of

@@ -10,8 +10,9 @@ Public API (mirrors the reference's task signatures):
 
 Drop-in task modules with the reference harness contract (``ModelNew``,
 ``get_inputs``, ``get_init_inputs``) live in ``tasks/``; the expert-parallel
-layer is in ``ep``, latent attention over a paged latent cache in ``attention``. Importing the package also registers the operators as
-``torch.ops.moe_b200.*`` (``torch_ops``).
+layer is in ``ep``, latent attention over a paged latent cache in ``attention``. Importing the package also
+registers the routing, expert, align and quantisation operators as ``torch.ops.moe_b200.*`` (``torch_ops``);
+``moe_decode`` and the latent operators are functions only, which ``torch.compile`` does not trace into.
 """
 
 from .ops import (  # noqa: F401

@@ -75,7 +75,7 @@ def _ints(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
 
 def latent_cache_write(cache: torch.Tensor, latent: torch.Tensor, k_rope: torch.Tensor, slots: torch.Tensor) -> None:
     """Writes latent [n, 512] and k_rope [n, 64] (rows of any pitch) to the cache slots
-    ``slots`` [n] = page * page_size + offset; negative slots are skipped. 16-bit caches take their
+    ``slots`` [n] = page * page_size + offset, each at most once; negative slots are skipped. 16-bit caches take their
     own dtype; an e4m3 cache takes bf16 and quantises each 128 latent values with the power-of-two
     scale of ``quantize_rows_fp8`` (non-finite values are kept as NaN and leave their block's scale
     alone; finite ones read back finite: those that would round to 2^128 take 15/16 of it). Slots past the cache are skipped and reported by ``check_device_status``."""

@@ -28,11 +28,12 @@
 // for non-finite values before the draft tokens; if there is one, the rows are computed again key by
 // key over visible keys, while the pair's other waits hold their limit (s_hold).
 //
-// Measured on the device, 74 requests of 2560 tokens: 16-bit pages 56 us with 128 heads (935 TFLOP/s, 0.57 of
-// the burst bf16 rate) and 55 us with 16 (3.95 TB/s, 0.60 of HBM); e4m3 pages 111 us with either.
+// Measured, 74 requests of 2560 tokens, join included: 16-bit pages 65.5 us with 128 heads (805 TFLOP/s, 0.49 of
+// the burst bf16 rate) and 61 us with 16 (3.6 TB/s, 0.54 of HBM); e4m3 pages 118 and 117 us.
 // 16-bit pages are bound by what L2 gives the SMs: a tile brings 272 KB into a pair's shared memory (144 KB of K
-// and, read again, 128 KB of V) in 2.0 us, over 74 pairs 10 TB/s; asking for lines in L2 ahead of the copies
-// made it slower. e4m3 pages are bound by the way of a slot from its copy over the widening warps to its MMAs.
+// and 128 KB of V, all of which lies in the K slots of the two CTAs already) in 2.0 us, over 74 pairs 10 TB/s; asking
+// for lines in L2 ahead of the copies made it slower. e4m3 pages are bound by the way of a slot from its copy over the
+// widening warps to its MMAs, with every code widened twice, for K and for V.
 #include "latent.h"
 
 #include <cuda_fp8.h>

@@ -19,7 +19,8 @@
 // The reference point of a row's exponentials follows its maximum only when that has moved by
 // more than 2^8: P then stays below 256 (exact range for both 16-bit types), the sum is fp32, and
 // O in TMEM is rescaled a few times per row instead of once per tile. P is rounded to the
-// inputs' type for the second product (as wide as V itself); l sums the unrounded values.
+// inputs' type for the second product (as wide as V itself; in fp16 the smallest are off by up to 2^-25 of the
+// reference's 1); l sums the unrounded values.
 //
 // Masked places: a score is replaced before the maximum is taken, so keys may hold anything.
 // V meets P = 0 in the MMA, and 0 * NaN is NaN, so warps 18-19 zero the V rows past the request's
@@ -31,9 +32,10 @@
 // What bounds it: per 128 keys and CTA the MMAs take 2560 clocks, the exponentials 2048 of the
 // 4-per-clock units of each SM quarter, so the two have to overlap all the time, and every fourth pair
 // of exponentials is taken off those units by a polynomial. What is left is the chain softmax, PV, QK of each
-// subtile, and power: 128 heads of one causal prompt of 7993 tokens take 2330-2740 us (955-1124
-// TFLOP/s by the box, 0.58-0.68 of the burst bf16 rate), ragged prompts of up to 1777 tokens 55 us, where a CTA's start and its
-// few tiles count.
+// subtile (P lies in S's columns): 128 heads of one causal prompt of 7993 tokens take 2500-2570 us (1020-1045 TFLOP/s,
+// 0.62-0.63 of the burst bf16 rate), 2.8 us per tile, with the power cap as the clocks' limit. Ragged prompts of up to
+// 1777 tokens take 55 us, the longest unit's 14 tiles most of it: units are not split over keys, and start by their place
+// in cu_q, not by length.
 #include "latent.h"
 
 namespace moe {
@@ -46,8 +48,9 @@ constexpr int kPfSlots = 8;
 constexpr int kSlotBytes = 16384;
 constexpr int kQSubBytes = 3 * 16384;    // a subtile of Q: three [128 rows][64] chunks
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial, beside the exponential units' three:
-                               // 7993 tokens of 128 heads 2690 us without, 2330 us with
+constexpr int kPolyEvery = 4;  // every fourth pair of exponentials by polynomial, beside the exponential units' three.
+                               // None, a quarter, a half in turn on one card, us: 7993 tokens of 128 heads 2594, 2555,
+                               // 2667; a piece of a context 88.6, 87.5, 90.0; ragged prompts 55.3, 55.1, 55.7
 
 struct PfSmem {
   static constexpr int kRing = 2 * kQSubBytes;

@@ -5,7 +5,8 @@
 //   out_t = sum_e w_te W2[e] a_te
 //
 // With a few tokens every chosen expert's weights are read for one or a handful of rows, so
-// the layer is bound by the bytes of the hit experts (3 * K * N each). The weights go from
+// the layer is bound by the bytes of the hit experts (3 * K * N each). They are read once per 8
+// pairs of an expert: with more than 8 tokens on one, again for the next 8. The weights go from
 // global memory straight into the registers of mma.sync.m16n8k16 as its A operand (16 weight
 // rows x 16 k), the tokens are its 8 columns: no shared memory, no barrier and no token tile
 // to fill on that way; a tcgen05 tile would pad 1..8 tokens to a 128-row operand and stage
@@ -29,9 +30,11 @@
 // few_down: one CTA per 16 rows of the output; its warps take consecutive runs of the (chunk, k
 //           block) list, add weight * product into their own shared rows in fp32, and the rows are
 //           summed in warp order.
-// Measured, of the bytes of the hit experts at HBM's 6.55 TB/s: e4m3, E 256, K 7168, N 2048: one token 90 us
-// (0.59; the conversions, and about 5 us of routing before the first load), 11 tokens 710-740 us (0.69-0.71); bf16, E 8, K 4096,
-// N 14336, 6 tokens 392-430 us (0.82-0.90).
+// Measured, of the bytes of the hit experts at HBM's 6.55 TB/s: e4m3, E 256, K 7168, N 2048: one token 91 us
+// (0.59: 65 up, 31 down, 1.3 to zero the maxima), 11 tokens 710-730 us (0.70-0.72); bf16, E 8, K 4096, N 14336, 6 tokens
+// 431-458 us (0.82-0.85). The warps wait for their loads: issue slots are 20 to 38 % busy, the integer pipe 18 to 34 %
+// with e4m3 weights. At 11 tokens (E 256) and 8 (E 8) moe_grouped_topk and moe_fused_experts(_fp8) have become faster, at
+// 32 tokens 1390 against 1670 us and 516 against 798; at E 64, K 2048, N 1408 they have not at 32 tokens (237 against 216).
 // Both give the same bits on every run. Sums are fp32; a_p is rounded once to the tokens' type (the
 // layer's other paths do the same).
 #include "common.cuh"

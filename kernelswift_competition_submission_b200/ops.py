@@ -537,22 +537,29 @@ def moe_layer(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, n
 
 
 def moe_decode_max_tokens(topk: int) -> int:
-    """The largest batch ``moe_decode`` takes: 32 tokens, fewer when topk is above 16."""
+    """The largest batch ``moe_decode`` takes: 32 tokens, fewer when topk is above 16. A limit of the kernels, not the
+    batch up to which they are the faster way (see ``moe_decode``)."""
     return int(_lib.load().moe_few_max_tokens(int(topk)))
 
 
 def moe_decode(hidden_states, gating_output, w1, w2, *, topk, renormalize=True, num_expert_group=1, topk_group=1,
                scoring_func="softmax", routed_scaling_factor=1.0, e_score_correction_bias=None, group_score=None,
                w1_scale=None, w2_scale=None, out=None, workspace=None):
-    """``moe_layer`` for the few tokens of a decode step, in two kernels that read every chosen
-    expert's weights once.
+    """``moe_layer`` for the few tokens of a decode step, in two kernels that read a chosen expert's
+    weights once per 8 of its tokens.
 
     hidden_states [M, K] (bf16 or fp16, M <= ``moe_decode_max_tokens(topk)``), gating_output
     [M, E]; w1 [E, 2N, K] and w2 [E, K, N] in the dtype of hidden_states, or e4m3 with fp32
     ``w1_scale`` / ``w2_scale`` per 128 x 128 block (``quantize_weights_fp8``). With e4m3 weights
     the tokens and SiLU*mul rows are used in 16 bits (``fused_moe_fp8`` quantises them to e4m3): fp16 as
     it is, bf16 as fp16 under a power of two per row, exact for values above 2^-28 of the
-    row's largest. Routing as ``grouped_topk``. Returns [M, K] in the dtype of hidden_states.
+    row's largest. Routing as ``grouped_topk``. Returns [M, K] in the dtype of hidden_states. Weights that are not
+    contiguous are copied on every call.
+
+    Measured against ``grouped_topk`` with ``fused_moe`` / ``fused_moe_fp8``, us: 256 e4m3 experts of K 7168, N 2048,
+    topk 8: 1 token 96 / 140, 4 tokens 287 / 343, 8 tokens 544 / 557, 11 tokens 720 / 695, 32 tokens 1670 / 1390;
+    8 bf16 experts of K 4096, N 14336, topk 2: 1 token 142 / 212, 6 tokens 450 / 446, 8 tokens 496 / 471, 32 tokens
+    798 / 516; 64 bf16 experts of K 2048, N 1408, topk 6: 1 token 39 / 70, 32 tokens 216 / 237.
     """
     name = "moe_decode"
     if scoring_func == "softmax":
