@@ -430,6 +430,13 @@ __device__ __forceinline__ void add_pair(float& d0, float& d1, float b0, float b
       : "f"(b0), "f"(b1));
 }
 
+// 2^x by the exponential unit
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---------------------------------------------------------------- element types
 template <typename T> struct ElemTraits;
 template <> struct ElemTraits<__nv_bfloat16> {
@@ -458,6 +465,7 @@ template <> struct ElemTraits<__half> {
 };
 
 __host__ __device__ constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---------------------------------------------------------------- e4m3 block scales
 // Scale of a block whose largest magnitude is amax, so that every code lands in

@@ -177,8 +177,6 @@ latent_cache_read_kernel(const uint8_t* __restrict__ cache, int64_t num_pages, i
   }
 }
 
-inline bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace moe
 
@@ -198,12 +196,12 @@ extern "C" int moe_latent_cache_write(int dtype, const void* latent, int64_t ld_
   if (!page_size_ok(page_size) || num_pages > INT32_MAX || num_tokens > (int64_t)INT32_MAX) return MOE_ERR_BAD_SHAPE;
   if (num_tokens == 0) return MOE_OK;
   if (!latent || !k_rope || !slots || !cache || ld_latent < 0 || ld_rope < 0) return MOE_ERR_INVALID_ARG;
-  if (!al16(cache) || (reinterpret_cast<uintptr_t>(latent) & 1u) || (reinterpret_cast<uintptr_t>(k_rope) & 1u) ||
+  if (!aligned16(cache) || (reinterpret_cast<uintptr_t>(latent) & 1u) || (reinterpret_cast<uintptr_t>(k_rope) & 1u) ||
       (reinterpret_cast<uintptr_t>(slots) & 7u))
     return MOE_ERR_INVALID_ARG;
   const int rc = moe_check_device();
   if (rc != MOE_OK) return rc;
-  const bool vl = al16(latent) && ld_latent % 8 == 0;
+  const bool vl = aligned16(latent) && ld_latent % 8 == 0;
   const bool vr = (reinterpret_cast<uintptr_t>(k_rope) & 3u) == 0 && ld_rope % 2 == 0;
   const unsigned blocks = (unsigned)ceil_div(num_tokens * 32, kCacheThreads);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -231,7 +229,7 @@ extern "C" int moe_latent_cache_read(int cache_fmt, const void* cache, int64_t n
   if (total == 0) return MOE_OK;
   if (!cache || !cu_lens || !latent || !k_rope || (num_seqs > 0 && table_width > 0 && !block_table))
     return MOE_ERR_INVALID_ARG;
-  if (!al16(cache) || !al16(latent) || !al16(k_rope)) return MOE_ERR_INVALID_ARG;
+  if (!aligned16(cache) || !aligned16(latent) || !aligned16(k_rope)) return MOE_ERR_INVALID_ARG;
   const int rc = moe_check_device();
   if (rc != MOE_OK) return rc;
   const unsigned blocks = (unsigned)ceil_div(total * 32, kCacheThreads);

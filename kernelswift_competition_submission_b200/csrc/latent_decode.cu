@@ -88,12 +88,6 @@ struct DcArgs {
   int* status;
 };
 
-__device__ __forceinline__ float ex2d(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ int clamped_len(const DcArgs& a, int b) {
   const int64_t cap = (int64_t)a.table_width << a.page_shift;
   const int64_t n = __ldg(a.lens + b);
@@ -749,7 +743,7 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const bool move = top > m_ref + kDcRescaleLog2 || m_ref == -INFINITY;
         float f = 1.0f;
         if (move) {
-          f = (m_ref == -INFINITY) ? 0.f : ex2d(m_ref - top);
+          f = (m_ref == -INFINITY) ? 0.f : ex2(m_ref - top);
           m_ref = top;
           l *= f;
         }
@@ -758,8 +752,8 @@ latent_decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2d(fmaf(__uint_as_float(raw[2 * e]), a.scale_log2, -base));
-          const float p1 = ex2d(fmaf(__uint_as_float(raw[2 * e + 1]), a.scale_log2, -base));
+          const float p0 = ex2(fmaf(__uint_as_float(raw[2 * e]), a.scale_log2, -base));
+          const float p1 = ex2(fmaf(__uint_as_float(raw[2 * e + 1]), a.scale_log2, -base));
           sum[e & 1] += p0;
           sum[2 + (e & 1)] += p1;
           p[e] = ElemTraits<T>::pack2(p0, p1);
@@ -934,7 +928,7 @@ latent_decode_join_kernel(const __grid_constant__ DcArgs a) {
     const int64_t s = place(p);
     const float2 ml = a.part_ml[s];
     if (ml.y == 0.f) continue;  // saw nothing; a NaN sum goes on
-    const float w = ex2d(ml.x - base);
+    const float w = ex2(ml.x - base);
     l += w * ml.y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1024,8 +1018,6 @@ cudaError_t launch_decode(int dtype, DcArgs a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-inline bool al16d(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 }  // namespace
 }  // namespace moe
 
@@ -1050,8 +1042,8 @@ extern "C" int moe_latent_decode(int dtype, const void* q, int64_t num_seqs, int
   if (num_seqs == 0) return MOE_OK;
   if (num_pages == 0 || !q || !cache || !cache_lens || !out || (table_width > 0 && !block_table))
     return MOE_ERR_INVALID_ARG;
-  if (!al16d(q) || !al16d(cache) || !al16d(out)) return MOE_ERR_INVALID_ARG;
-  if (workspace_bytes < moe_latent_decode_workspace_bytes(num_seqs, q_len, heads) || !workspace || !al16d(workspace))
+  if (!aligned16(q) || !aligned16(cache) || !aligned16(out)) return MOE_ERR_INVALID_ARG;
+  if (workspace_bytes < moe_latent_decode_workspace_bytes(num_seqs, q_len, heads) || !workspace || !aligned16(workspace))
     return MOE_ERR_WORKSPACE;
   const int rc = moe_check_device();
   if (rc != MOE_OK) return rc;

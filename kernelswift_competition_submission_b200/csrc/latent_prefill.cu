@@ -83,12 +83,6 @@ struct PfArgs {
   int* status;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // 2^x of two values x <= 2^7 without the exponential unit: x = n + f with n the nearest integer, 2^f by its
 // degree-4 polynomial of least relative error on [-1/2, 1/2] (2.7e-6 in fp32; a weighted least-squares fit at
 // Chebyshev nodes iterated to equal extrema), times 2^n made from n's bits. n stops at -127, whose bits are
@@ -615,8 +609,6 @@ latent_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   }
 }
 
-inline bool al16p(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 template <typename T>
 cudaError_t launch_prefill(int dtype, PfArgs a, cudaStream_t st) {
   CUtensorMap mq, mkv, mkr, mv;
@@ -659,7 +651,7 @@ extern "C" int moe_latent_prefill(int dtype, const void* q, int64_t q_stride_t, 
     return MOE_ERR_BAD_SHAPE;
   if (total_q == 0) return MOE_OK;
   if (!q || !cu_q || !cu_k || !out || (total_k > 0 && (!kv || !k_rope))) return MOE_ERR_INVALID_ARG;
-  if (!al16p(q) || !al16p(kv) || !al16p(k_rope) || !al16p(out)) return MOE_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(kv) || !aligned16(k_rope) || !aligned16(out)) return MOE_ERR_INVALID_ARG;
   // 16-byte TMA strides above zero; the stride of a dimension of one is not used
   int64_t st[5] = {total_q > 1 ? q_stride_t : 8, heads > 1 ? q_stride_h : 8, total_k > 1 ? kv_stride_t : 8,
                    heads > 1 ? kv_stride_h : 8, total_k > 1 ? kr_stride_t : 8};

@@ -555,8 +555,6 @@ few_down_kernel(const T* __restrict__ act, const FewTables* __restrict__ tab, co
 }
 
 inline size_t few_tables_bytes() { return (sizeof(FewTables) + 255) / 256 * 256; }
-inline bool al16f(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 template <typename T, bool F8>
 cudaError_t launch_few(const void* x, int64_t ld_x, const FewRouting& rt, const void* w1, const float* w1s,
                        const void* w2, const float* w2s, int M, int E, int K, int N, void* out, void* ws,
@@ -627,14 +625,14 @@ extern "C" int moe_few_tokens(int dtype, const void* hidden_states, int64_t ld_h
   if (num_tokens == 0) return MOE_OK;
   if (!hidden_states || !gating_output || !w1 || !w2 || !out || !workspace || (weight_e4m3 && (!w1_scale || !w2_scale)))
     return MOE_ERR_INVALID_ARG;
-  if (!al16f(hidden_states) || ld_hidden % 8 || ld_hidden < 0 || !al16f(w1) || !al16f(w2) || !al16f(workspace))
+  if (!aligned16(hidden_states) || ld_hidden % 8 || ld_hidden < 0 || !aligned16(w1) || !aligned16(w2) || !aligned16(workspace))
     return MOE_ERR_INVALID_ARG;
   if (workspace_bytes < moe_few_workspace_bytes(num_tokens, topk, intermediate_size)) return MOE_ERR_WORKSPACE;
   const int rc = moe_check_device();
   if (rc != MOE_OK) return rc;
   const FewRouting rt{gating_output, bias,         topk,           renormalize, num_expert_group, topk_group,
                       scoring_func,  group_score_mode, routed_scaling_factor,
-                      al16f(gating_output) && (!bias || al16f(bias))};
+                      aligned16(gating_output) && (!bias || aligned16(bias))};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int M = (int)num_tokens;
   cudaError_t err;
